@@ -10,6 +10,7 @@ from __future__ import annotations
 import concurrent.futures
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -38,16 +39,23 @@ def _nvcc() -> str:
     return nvcc
 
 
-def _sources_digest() -> str:
-    h = hashlib.sha256()
-    names = sorted(os.listdir(CSRC)) + ["../../include/recflex_b200.h"]
-    for name in names:
-        path = os.path.normpath(os.path.join(CSRC, name))
-        if os.path.isfile(path):
-            h.update(name.encode())
-            with open(path, "rb") as f:
-                h.update(f.read())
-    h.update(" ".join(NVCC_FLAGS).encode())
+_INCLUDE = re.compile(r'^\s*#\s*include\s+"([^"]+)"', re.M)
+
+
+def _unit_digest(unit) -> str:
+    """Digest of what an object is built from: its source, the headers that it includes by quotes, and the flags."""
+    _, src, extra = unit
+    h = hashlib.sha256(" ".join(NVCC_FLAGS + extra).encode())
+    todo, seen = [os.path.join(CSRC, src)], set()
+    while todo:
+        path = os.path.normpath(todo.pop())
+        if path in seen or not os.path.isfile(path):
+            continue
+        seen.add(path)
+        with open(path, "rb") as f:
+            text = f.read()
+        h.update(os.path.basename(path).encode() + text)
+        todo += [os.path.join(os.path.dirname(path), name) for name in sorted(_INCLUDE.findall(text.decode()))]
     return h.hexdigest()
 
 
@@ -59,15 +67,20 @@ def _units():
         ("eb_noalloc.o", "eb_noalloc.cu", []),
         ("eb_warp.o", "eb_warp_inst.cu", []),
         ("eb_longbag.o", "eb_longbag_inst.cu", []),
+        ("eb_rows.o", "eb_rows.cu", []),
+        ("eb_linear.o", "eb_linear.cu", []),
     ]
     for occ in range(1, 9):
         units.append((f"eb_fused_occ{occ}.o", "eb_fused_inst.cu", [f"-DEB_OCC={occ}"]))
     return [u for u in units if os.path.exists(os.path.join(CSRC, u[1]))]
 
 
-def _compile(unit, verbose: bool) -> str:
+def _compile(unit, force: bool, verbose: bool) -> str:
     obj, src, extra = unit
     out = os.path.join(BUILD_DIR, obj)
+    stamp, digest = out + ".sha256", _unit_digest(unit)
+    if not force and os.path.exists(out) and _read(stamp) == digest:
+        return digest
     cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", INCLUDE_DIR, "-c", os.path.join(CSRC, src), "-o", out]
     if verbose:
         cmd.insert(1, "-Xptxas")
@@ -77,22 +90,31 @@ def _compile(unit, verbose: bool) -> str:
         raise RuntimeError(f"nvcc failed for {src} {extra}:\n{res.stdout}\n{res.stderr}")
     if verbose:
         sys.stderr.write(res.stderr)
-    return out
+    with open(stamp, "w") as f:
+        f.write(digest)
+    return digest
+
+
+def _read(path: str) -> str:
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read().strip()
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile (if sources changed) and return the path of the shared library."""
-    os.makedirs(BUILD_DIR, exist_ok=True)
-    stamp = os.path.join(BUILD_DIR, "sources.sha256")
-    digest = _sources_digest()
-    if not force and os.path.exists(LIB_PATH) and os.path.exists(stamp):
-        with open(stamp) as f:
-            if f.read().strip() == digest:
-                return LIB_PATH
+    """Compile the units whose sources changed, link, and return the path of the shared library."""
     units = _units()
+    stamp = os.path.join(BUILD_DIR, "sources.sha256")
+    # checked before anything is written: several processes may ask for an up-to-date library at once
+    digest = hashlib.sha256(" ".join(_unit_digest(u) for u in units).encode()).hexdigest()
+    if not force and os.path.exists(LIB_PATH) and _read(stamp) == digest:
+        return LIB_PATH
+    os.makedirs(BUILD_DIR, exist_ok=True)
     jobs = jobs or min(len(units), os.cpu_count() or 1)
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
-        objs = list(pool.map(lambda u: _compile(u, verbose), units))
+        list(pool.map(lambda u: _compile(u, force, verbose), units))
+    objs = [os.path.join(BUILD_DIR, u[0]) for u in units]
     cmd = [_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB_PATH, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
