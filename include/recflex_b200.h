@@ -487,6 +487,102 @@ int eb_forward_packed_noalloc(int device, int num_features, const int64_t* rows,
                               int64_t out_ld, void* stream);
 int eb_noalloc_check_status(int device, void* stream);
 
+/*
+ * Dense layers behind the pooled rows (no counterpart in the reference, whose
+ * RecomModel runs torch.nn.Linear, RecFlex/rec_modules.py:143-179): rows in 8
+ * bits, their matrix product, rows by expert, and matrix products grouped by
+ * expert.  None of them allocates or synchronises (eb_linear_check_status
+ * does); every launch goes to `stream`, and calls on different streams share
+ * nothing but the buffers that the caller passes to both.  All of them may be
+ * captured into a graph.
+ */
+
+/* element types of the rows: EB_OUT_F32, EB_OUT_BF16, EB_OUT_F16 as above, and signed bytes */
+#define EB_ROW_I8 3
+/* activation of a layer, applied in 32 bits before its result is rounded */
+#define EB_ACT_NONE 0
+#define EB_ACT_RELU 1
+#define EB_ACT_SIGMOID 2
+/* largest number of experts of a call, and longest row of an 8-bit product (2^31 / 2^14 terms fit the 32-bit sums) */
+#define EB_MAX_GROUPS 1024
+#define EB_MAX_I8_COLS 131071
+
+/*
+ * Rows in 8 bits with one scale a row: scale[r] = max|x[r, :]| / 127, rounded
+ * to fp32, and q[r, c] = x[r, c] / scale[r] (that rounded scale; the exact
+ * quotient) to the nearest integer, ties to even, within [-127, 127].  A row of
+ * zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has
+ * codes 0 and that infinity or a NaN as its scale, so that products with it are
+ * NaN.  x is [rows, cols] of x_dtype (EB_OUT_*) with rows x_ld elements apart,
+ * q [rows, cols] signed bytes with rows q_ld bytes apart; any alignment (rows
+ * on 16-byte boundaries are read with wide loads).
+ */
+int eb_quantize_rows(const void* x, int64_t rows, int64_t cols, int64_t x_ld, int x_dtype, void* q, int64_t q_ld,
+                     float* scale, int device, void* stream);
+
+/*
+ * Rows by expert: `groups` holds one expert number per row (EB_I32 or EB_I64).
+ * Writes `order` (rows entries): the row numbers, expert by expert, each
+ * expert's rows in increasing order, then the rows whose number lies outside
+ * [0, num_groups); and `offsets` (num_groups + 1 entries, from 0): expert g owns
+ * order[offsets[g] .. offsets[g + 1]).  The result is the same on every run.
+ * At most EB_MAX_GROUPS experts and 2^31 - 1 rows.  `workspace` needs the bytes
+ * that eb_group_rows_workspace_bytes reports (8-byte aligned, any contents; may
+ * be NULL when that is 0).
+ */
+int eb_group_rows_workspace_bytes(int64_t rows, int num_groups, size_t* bytes);
+int eb_group_rows(const void* groups, int64_t rows, int num_groups, int index_dtype, int32_t* order, int32_t* offsets,
+                  void* workspace, size_t workspace_bytes, int device, void* stream);
+
+/*
+ * One layer's matrix products.  Position i of `positions` belongs to the group
+ * g with offsets[g] <= i < offsets[g + 1] (one group of all positions when
+ * offsets is NULL); with s = in_rows[i] and d = out_rows[i] (i itself where the
+ * list is NULL)
+ *
+ *   out[d, :] = activation(x[s, :] . weight[g]^T * scales + bias[g, :])
+ *
+ * where scales is 1, or x_scale[s] * w_scale[g, n] for EB_ROW_I8.  Products
+ * are summed in fp32 (EB_OUT_BF16, EB_OUT_F16) or exactly in 32-bit integers
+ * (EB_ROW_I8), and rounded once to out_dtype.
+ *
+ * Positions of no group (in front of offsets[0], or behind the last offset)
+ * leave their output rows as they were, or get rows of zeros with zero_rest.
+ * Entries of in_rows outside [0, x_rows) give a product with a row of zeros,
+ * entries of out_rows outside [0, out_rows_total) are not stored, offsets that
+ * decrease or leave [0, positions] are clamped; each sets a bit of *status.
+ * Row numbers in out_rows must differ from one another.
+ */
+typedef struct eb_linear_args {
+  const void* x;           /* [x_rows, k] of dtype, rows x_ld elements apart */
+  const void* weight;      /* [num_groups, n, k] of dtype, rows w_ld and groups w_group_ld elements apart */
+  const float* bias;       /* [num_groups, n] or NULL */
+  const float* x_scale;    /* EB_ROW_I8: [x_rows] */
+  const float* w_scale;    /* EB_ROW_I8: [num_groups, n] */
+  const int32_t* offsets;  /* [num_groups + 1] or NULL */
+  const int32_t* in_rows;  /* [positions] or NULL */
+  const int32_t* out_rows; /* [positions] or NULL */
+  void* out;               /* [out_rows_total, n] of out_dtype, rows out_ld elements apart */
+  uint32_t* status;        /* device word, zero before its first use; calls only set bits in it */
+  int64_t x_rows, x_ld, w_ld, w_group_ld, positions, out_rows_total, out_ld;
+  int32_t n, k, num_groups;
+  int32_t dtype;           /* of x and weight: EB_OUT_BF16, EB_OUT_F16 or EB_ROW_I8 */
+  int32_t out_dtype;       /* EB_OUT_F32 (only with EB_ROW_I8), EB_OUT_BF16 or EB_OUT_F16; `dtype` itself when that is a float */
+  int32_t activation;      /* EB_ACT_* */
+  int32_t zero_rest;
+} eb_linear_args;
+
+/*
+ * x and weight must start on 16-byte boundaries with x_ld, w_ld and w_group_ld
+ * multiples of 16 bytes (EB_ERR_UNSUPPORTED otherwise).  Fewer than 2^31
+ * positions and rows.
+ */
+int eb_linear(const eb_linear_args* args, int device, void* stream);
+
+/* Reads and clears the status word of eb_linear: EB_ERR_BAD_INPUT for bad offsets or row numbers, EB_ERR_CUDA when a
+ * kernel gave up waiting for its own copies.  Synchronises `stream`. */
+int eb_linear_check_status(uint32_t* status, int device, void* stream);
+
 /* Message of the calling thread's last failure ("" if none). */
 const char* eb_last_error(void);
 

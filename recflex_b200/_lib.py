@@ -22,6 +22,10 @@ EB_ERR_TOO_LARGE = -6
 EB_F32, EB_F16 = 0, 1
 EB_I32, EB_I64 = 0, 1
 EB_OUT_F32, EB_OUT_BF16, EB_OUT_F16 = 0, 1, 2
+EB_ROW_I8 = 3
+EB_ACT_NONE, EB_ACT_RELU, EB_ACT_SIGMOID = 0, 1, 2
+EB_MAX_GROUPS = 1024
+EB_MAX_I8_COLS = 131071
 EB_EXCHANGE_COPY_ENGINES, EB_EXCHANGE_SM_PUSH = 0, 1
 EB_NOALLOC_MAX_FEATURES = 1024
 EB_SCHED_AUTO, EB_SCHED_GROUP, EB_SCHED_WARP, EB_SCHED_FLAT, EB_SCHED_STREAM, EB_SCHED_PIPE = 0, 1, 2, 3, 4, 5
@@ -39,6 +43,17 @@ class EbSchedule(C.Structure):
         ("vec_bytes", C.c_int32),
         ("bags_per_tile", C.c_int32),
     ]
+
+
+class EbLinearArgs(C.Structure):
+    """Mirror of `eb_linear_args`."""
+
+    _fields_ = [(name, C.c_void_p) for name in ("x", "weight", "bias", "x_scale", "w_scale", "offsets", "in_rows",
+                                                "out_rows", "out", "status")] + \
+               [(name, C.c_int64) for name in ("x_rows", "x_ld", "w_ld", "w_group_ld", "positions", "out_rows_total",
+                                               "out_ld")] + \
+               [(name, C.c_int32) for name in ("n", "k", "num_groups", "dtype", "out_dtype", "activation",
+                                               "zero_rest")]
 
 
 class EbError(RuntimeError):
@@ -102,6 +117,13 @@ PROTOTYPES = {
                                       C.POINTER(C.c_int64), C.c_int, C.c_int, C.c_void_p, C.c_int64,
                                       C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int,
                                       C.c_void_p, C.c_size_t, C.c_void_p, C.POINTER(C.c_void_p), C.c_int]),
+    "eb_quantize_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int64,
+                                   C.c_void_p, C.c_int, C.c_void_p]),
+    "eb_group_rows_workspace_bytes": (C.c_int, [C.c_int64, C.c_int, C.POINTER(C.c_size_t)]),
+    "eb_group_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                C.c_size_t, C.c_int, C.c_void_p]),
+    "eb_linear": (C.c_int, [C.POINTER(EbLinearArgs), C.c_int, C.c_void_p]),
+    "eb_linear_check_status": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
     "eb_last_error": (C.c_char_p, []),
     "eb_version": (C.c_char_p, []),
 }

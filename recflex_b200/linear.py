@@ -1,0 +1,327 @@
+"""Dense layers behind the pooled rows: rows in 8 bits, their matrix product, rows by expert, products by expert.
+
+The reference's model runs `torch.nn.Linear` on the pooled rows (RecFlex/rec_modules.py:143-179) and has none of
+these.  All of them call librecflex_b200.so (`eb_quantize_rows`, `eb_linear`, `eb_group_rows`) on the current stream,
+never synchronise with the host, and may be captured into a CUDA graph once one of them has run on the device.
+
+They are forward only, like the embedding layer in front of them: an argument that requires a gradient is refused
+while gradients are being recorded.  Row numbers and offsets live on the GPU and are checked there: bad ones never
+fault, and `check_status` reports them.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import threading
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+
+MAX_GROUPS = _lib.EB_MAX_GROUPS
+_FLOATS = {torch.float32: _lib.EB_OUT_F32, torch.bfloat16: _lib.EB_OUT_BF16, torch.float16: _lib.EB_OUT_F16}
+_ACTIVATIONS = {"none": _lib.EB_ACT_NONE, "relu": _lib.EB_ACT_RELU, "sigmoid": _lib.EB_ACT_SIGMOID}
+_INDEX = {torch.int32: _lib.EB_I32, torch.int64: _lib.EB_I64}
+
+_status_lock = threading.Lock()
+_status = {}
+
+
+def _status_word(device: torch.device) -> torch.Tensor:
+    """The device's status word, made at the first call.  Calls only set bits in it, so all streams share it."""
+    word = _status.get(device)
+    if word is None:
+        with _status_lock:
+            word = _status.get(device)
+            if word is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first call on a device must come before any stream capture")
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+                torch.cuda.current_stream(device).synchronize()
+                _status[device] = word
+    return word
+
+
+def check_status(device=None) -> None:
+    """Raise if a product since the last check met offsets or row numbers outside their range (synchronises)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    word = _status.get(device)
+    if word is not None:
+        _lib.check(_lib.load().eb_linear_check_status(word.data_ptr(), device.index,
+                                                      torch.cuda.current_stream(device).cuda_stream))
+
+
+def _check(name: str, t: torch.Tensor, dims: int, dtypes, device: Optional[torch.device] = None) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must live on {device}, it lives on {t.device}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, it has {t.dim()}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: these layers are forward only (detach it or use torch.no_grad())")
+
+
+def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    _check(name, t, len(shape), (dtype,), device)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, it is {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _has_wide_rows(t: torch.Tensor) -> bool:
+    """Rows on 16-byte boundaries that do not overlap, as the products read them."""
+    size, k = t.element_size(), t.shape[-1]
+    if t.data_ptr() % 16 or (t.stride(-1) != 1 and k > 1):
+        return False
+    least = k
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] > 1 and (t.stride(d) * size % 16 or t.stride(d) < least):
+            return False
+        if t.shape[d] > 1:
+            least = t.stride(d) * (t.shape[d] - 1) + least
+    return True
+
+
+def _empty_wide(shape, dtype: torch.dtype, device) -> torch.Tensor:
+    """Uninitialised [..., k] whose rows start on 16-byte boundaries."""
+    per = 16 // dtype.itemsize
+    k = shape[-1]
+    return torch.empty(tuple(shape[:-1]) + ((k + per - 1) // per * per,), dtype=dtype, device=device)[..., :k]
+
+
+def pack_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [..., k] as it is if its rows start on 16-byte boundaries, otherwise a copy whose rows do.  The products
+    take any layout and make this copy themselves; weights are better laid out once."""
+    if _has_wide_rows(t):
+        return t
+    return _empty_wide(t.shape, t.dtype, t.device).copy_(t)
+
+
+def _row_stride(t: torch.Tensor, dim: int) -> int:
+    """Elements between neighbours of `dim`; where there is one entry only, what a packed tensor has."""
+    if t.shape[dim] > 1:
+        return t.stride(dim)
+    per = 16 // t.element_size()
+    if dim == t.dim() - 2:
+        return (t.shape[-1] + per - 1) // per * per
+    return _row_stride(t, dim + 1) * max(1, t.shape[dim + 1])
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows in 8 bits with one scale a row: `(q, scale)` with `q` int8 `[rows, k]`, `scale` float32 `[rows]`.
+
+    `scale = max|x| / 127` of the row, and `q` the nearest integer (ties to even) to `x / scale`.  A row of zeros has
+    scale 0; a row that holds an infinity or a NaN has codes 0 and a scale that is not finite, so that its products are
+    NaN.  `x`: `[rows, k]` float32, bfloat16 or float16 with any strides.  The rows of `q` start on 16-byte boundaries.
+    """
+    _check("x", x, 2, _FLOATS)
+    rows, k = x.shape
+    if k > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < k:
+        x = x.contiguous()
+    q = _empty_wide((rows, k), torch.int8, x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _lib.check(_lib.load().eb_quantize_rows(x.data_ptr(), rows, k, x.stride(0) if rows > 1 else k, _FLOATS[x.dtype],
+                                            q.data_ptr(), q.stride(0) if rows > 1 else k, scale.data_ptr(),
+                                            x.device.index, _stream(x.device)))
+    return q, scale
+
+
+def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows by expert: `(order, offsets)`, both int32.
+
+    `groups`: `[rows]` int32 or int64 expert numbers.  `order` lists the row numbers expert by expert, each expert's
+    rows in increasing order, then the rows whose number lies outside `[0, num_groups)` (-1 for padding, say).  Expert
+    g owns `order[offsets[g]:offsets[g + 1]]`: the `offsets` that `grouped_linear` takes.
+    """
+    _check("groups", groups, 1, _INDEX)
+    if not groups.is_contiguous():
+        groups = groups.contiguous()
+    rows, device, lib = groups.numel(), groups.device, _lib.load()
+    need = C.c_size_t()
+    _lib.check(lib.eb_group_rows_workspace_bytes(rows, int(num_groups), C.byref(need)))
+    order = torch.empty(rows, dtype=torch.int32, device=device)
+    offsets = torch.empty(int(num_groups) + 1, dtype=torch.int32, device=device)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _lib.check(lib.eb_group_rows(groups.data_ptr(), rows, int(num_groups), _INDEX[groups.dtype], order.data_ptr(),
+                                 offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, device.index,
+                                 _stream(device)))
+    return order, offsets
+
+
+def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out):
+    device = x.device
+    groups, n, k = weight.shape if weight.dim() == 3 else (1,) + tuple(weight.shape)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    if x.shape[1] != k:
+        raise ValueError(f"x has {x.shape[1]} columns, weight has {k}")
+    if n < 1 or k < 1 or groups < 1:
+        raise ValueError(f"weight must not be empty, it is {list(weight.shape)}")
+    a = _lib.EbLinearArgs()
+    keep = []  # alive until the launch is on the stream
+    positions = x.shape[0]
+    if in_rows is not None:
+        _check("in_rows", in_rows, 1, (torch.int32,), device)
+        keep.append(in_rows.contiguous())
+        positions, a.in_rows = in_rows.numel(), keep[-1].data_ptr()
+    if out_rows is not None:
+        _check("out_rows", out_rows, 1, (torch.int32,), device)
+        if out_rows.numel() != positions:
+            raise ValueError(f"out_rows has {out_rows.numel()} entries for {positions} rows")
+        keep.append(out_rows.contiguous())
+        a.out_rows = keep[-1].data_ptr()
+    if offsets is not None:
+        keep.append(_vector("offsets", offsets, (groups + 1,), torch.int32, device))
+        a.offsets = keep[-1].data_ptr()
+    lead = (groups, n) if weight.dim() == 3 else (n,)
+    if bias is not None:
+        keep.append(_vector("bias", bias, lead, torch.float32, device))
+        a.bias = keep[-1].data_ptr()
+    if x.dtype == torch.int8:
+        if x_scale is None or weight_scale is None:
+            raise ValueError("8-bit products need x_scale and weight_scale")
+        keep.append(_vector("x_scale", x_scale, (x.shape[0],), torch.float32, device))
+        a.x_scale = keep[-1].data_ptr()
+        keep.append(_vector("weight_scale", weight_scale, lead, torch.float32, device))
+        a.w_scale = keep[-1].data_ptr()
+        a.dtype = _lib.EB_ROW_I8
+        out_dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
+    else:
+        if x_scale is not None or weight_scale is not None:
+            raise ValueError("scales belong to 8-bit products only")
+        if out_dtype not in (None, x.dtype):
+            raise TypeError(f"products of {x.dtype} give {x.dtype}, not {out_dtype}")
+        out_dtype = x.dtype
+        a.dtype = _FLOATS[x.dtype]
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if out is None:
+        # without out_rows every position is a row of the result, and the kernel fills those of no group with zeros
+        make = torch.empty if out_rows is None else torch.zeros
+        out = make((positions, n), dtype=out_dtype, device=device)
+        a.zero_rest = int(out_rows is None)
+    else:
+        _check("out", out, 2, (out_dtype,), device)
+        if out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
+            raise ValueError(f"out must be [rows, {n}] with unit column stride and rows that do not overlap")
+        if out_rows is None and out.shape[0] < positions:
+            raise ValueError(f"out has {out.shape[0]} rows for {positions}")
+        lo, hi = _span(out)
+        for t in (x, weight):
+            first, last = _span(t)
+            if first < hi and lo < last:
+                raise ValueError("out must not share memory with the arguments")
+    x, weight = pack_rows(x), pack_rows(weight)
+    a.x, a.weight, a.out, a.status = x.data_ptr(), weight.data_ptr(), out.data_ptr(), _status_word(device).data_ptr()
+    a.x_rows, a.x_ld = x.shape[0], _row_stride(x, 0)
+    a.w_ld, a.w_group_ld = _row_stride(weight, weight.dim() - 2), _row_stride(weight, 0)
+    a.positions, a.out_rows_total = positions, out.shape[0]
+    a.out_ld = out.stride(0) if out.shape[0] > 1 else n
+    a.n, a.k, a.num_groups = n, k, groups
+    a.out_dtype, a.activation = _FLOATS[out_dtype], _ACTIVATIONS[activation]
+    _lib.check(_lib.load().eb_linear(C.byref(a), device.index, _stream(device)))
+    return out
+
+
+def int8_linear(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, activation: str = "none",
+                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`activation((q @ weight.T) * q_scale[:, None] * weight_scale + bias)` of 8-bit rows and weights.
+
+    `q` int8 `[rows, k]` and `q_scale` float32 `[rows]` as `quantize_rows` gives them; `weight` int8 `[n, k]`,
+    `weight_scale` float32 `[n]`; `bias` float32 `[n]`.  The products are summed exactly in 32-bit integers (k up to
+    131071), scaled in fp32 and rounded once to `out_dtype` (float32, bfloat16, the default, or float16).
+    """
+    _check("q", q, 2, (torch.int8,))
+    _check("weight", weight, 2, (torch.int8,), q.device)
+    return _product(q, weight, bias, activation, q_scale, weight_scale, None, None, None, out_dtype, out)
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   activation: str = "none", in_rows: Optional[torch.Tensor] = None,
+                   out_rows: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
+                   weight_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One matrix product per expert over ragged runs of rows:
+    `out[out_rows[i]] = activation(x[in_rows[i]] @ weight[g].T + bias[g])` for `offsets[g] <= i < offsets[g + 1]`.
+
+    `x` `[rows, k]` bfloat16 or float16 (summed in fp32, result of the same type), or int8 with `x_scale` float32
+    `[rows]` (result bfloat16 unless `out_dtype` says otherwise); `weight` `[experts, n, k]` of the same type, with
+    `weight_scale` float32 `[experts, n]` for int8; `bias` float32 `[experts, n]`; `offsets` int32 `[experts + 1]`,
+    `in_rows` and `out_rows` int32 row numbers (i itself where a list is not given).  `group_rows` makes both.
+
+    Positions of no expert (behind the last offset, or in front of the first) give rows of zeros when the result is
+    allocated here, and leave the rows of a given `out` as they were.  No row number may stand twice in `out_rows`.
+    """
+    _check("x", x, 2, (torch.bfloat16, torch.float16, torch.int8))
+    _check("weight", weight, 3, (x.dtype,), x.device)
+    if offsets is None:
+        raise ValueError("offsets must be an int32 tensor")
+    return _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out)
+
+
+class Int8Linear(nn.Module):
+    """A linear layer in 8 bits: `weight` `[n, k]` is quantised once, one scale per output unit; every call quantises
+    its rows, one scale per row, and multiplies 8-bit integers.  The result has the type of the argument."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none"):
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        q, scale = quantize_rows(weight.detach())
+        self.activation = activation
+        self.register_buffer("weight", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().float())
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        q, scale = quantize_rows(x)
+        return int8_linear(q, scale, self.weight, self.weight_scale, self.bias, self.activation, x.dtype)
+
+
+class GroupedLinear(nn.Module):
+    """One linear layer per expert: `weight` `[experts, n, k]` in bfloat16 or float16, `bias` `[experts, n]`.
+
+    `forward(x, offsets, in_rows, out_rows)` is `grouped_linear`.  `quantize()` turns the weights into 8 bits with one
+    scale per expert and output unit; from then on every call quantises its rows."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none"):
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        _check("weight", weight.detach(), 3, (torch.bfloat16, torch.float16))
+        self.activation = activation
+        self.register_buffer("weight", pack_rows(weight.detach()))
+        self.register_buffer("weight_scale", None)
+        self.register_buffer("bias", None if bias is None else bias.detach().float())
+
+    def quantize(self) -> "GroupedLinear":
+        if self.weight.dtype != torch.int8:
+            experts, n, k = self.weight.shape
+            q, scale = quantize_rows(self.weight.reshape(experts * n, k))
+            self.weight = q.unflatten(0, (experts, n))
+            self.weight_scale = scale.view(experts, n)
+        return self
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor, in_rows: Optional[torch.Tensor] = None,
+                out_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.weight.dtype != torch.int8:
+            return grouped_linear(x, self.weight, offsets, self.bias, self.activation, in_rows, out_rows)
+        q, scale = quantize_rows(x)
+        return grouped_linear(q, self.weight, offsets, self.bias, self.activation, in_rows, out_rows, scale,
+                              self.weight_scale, x.dtype)

@@ -24,6 +24,7 @@ import torch.nn as nn
 
 from . import _lib
 from ._lib import EbSchedule
+from .linear import MAX_GROUPS, GroupedLinear, Int8Linear, group_rows
 
 
 def _device_index(device) -> int:
@@ -477,22 +478,85 @@ class RecomModel(nn.Module):
     `mlp_dtype` (not in the reference, whose model is fp32 throughout) selects the MLP's precision.  With
     torch.bfloat16 or torch.float16 the embedding layer writes its pooled sums directly in that type
     (`FeatEmbed.set_output_dtype`), i.e. in the first linear layer's input layout and dtype: no fp32 intermediate is
-    written or re-read, and the cast costs nothing."""
+    written or re-read, and the cast costs nothing.
+
+    `num_experts` (not in the reference) > 0 gives the model that many MLPs over the one embedding, and `forward` takes
+    an expert number per sample: the batch is brought into expert order by row numbers only, the first layer reads the
+    pooled rows through them and the last one writes the scores back in batch order.  Samples whose number lies outside
+    [0, num_experts) score 0.  Needs a 16-bit `mlp_dtype`.
+
+    `quantize_mlp()` turns a model's trained layers into 8-bit ones (`linear.Int8Linear`)."""
 
     def __init__(self, mlp_unit_nums: List[int], device, embed_tables: Optional[List[torch.Tensor]] = None,
-                 table_shapes: Optional[Sequence[Tuple[int, int]]] = None, mlp_dtype: torch.dtype = torch.float32):
+                 table_shapes: Optional[Sequence[Tuple[int, int]]] = None, mlp_dtype: torch.dtype = torch.float32,
+                 num_experts: int = 0):
         super().__init__()
+        if num_experts < 0 or num_experts > MAX_GROUPS:
+            raise ValueError(f"num_experts must lie in [0, {MAX_GROUPS}], got {num_experts}")
+        if num_experts and mlp_dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"experts need a bfloat16 or float16 MLP, got {mlp_dtype}")
         self.device = torch.device("cuda", _device_index(device))
         self.embed_layer = FeatEmbed(device=self.device, embed_tables=embed_tables, table_shapes=table_shapes)
         self.embed_layer.set_output_dtype(mlp_dtype)
+        self.num_experts = int(num_experts)
         layers = []
         unit_nums = [self.embed_layer.output_units] + list(mlp_unit_nums) + [1]
         for i in range(len(unit_nums) - 1):
+            last = i + 2 == len(unit_nums)
+            if self.num_experts:
+                # the bounds of nn.Linear's own initial values
+                bound = 1.0 / max(1, unit_nums[i]) ** 0.5
+                weight = torch.empty((self.num_experts, unit_nums[i + 1], unit_nums[i]), dtype=mlp_dtype, device=self.device)
+                bias = torch.empty((self.num_experts, unit_nums[i + 1]), device=self.device)
+                layers.append(GroupedLinear(weight.uniform_(-bound, bound), bias.uniform_(-bound, bound),
+                                            "sigmoid" if last else "relu"))
+                continue
             layers.append(nn.Linear(unit_nums[i], unit_nums[i + 1], bias=True, device=self.device, dtype=mlp_dtype))
-            layers.append(nn.Sigmoid() if i + 2 == len(unit_nums) else nn.ReLU())
+            layers.append(nn.Sigmoid() if last else nn.ReLU())
         self.mlp = nn.Sequential(*layers)
 
+    def quantize_mlp(self) -> "RecomModel":
+        """Layers in 8 bits from here on: one scale per output unit, fixed now, and one per sample and layer, found by
+        every call.  Activations between the layers keep the model's `mlp_dtype`."""
+        layers = list(self.mlp)
+        if self.num_experts:
+            for layer in layers:
+                layer.quantize()
+            return self
+        done, names = [], {nn.ReLU: "relu", nn.Sigmoid: "sigmoid"}
+        for i, layer in enumerate(layers):
+            if isinstance(layer, nn.Linear):
+                after = names.get(type(layers[i + 1])) if i + 1 < len(layers) else None
+                done.append(Int8Linear(layer.weight, layer.bias, after or "none"))
+            elif not (type(layer) in names and i > 0 and isinstance(layers[i - 1], nn.Linear)):
+                done.append(layer)
+        self.mlp = nn.Sequential(*done)
+        return self
+
+    def _embed(self, values, offsets, include_last_offset):
+        """The pooled rows on 16-byte boundaries, as the grouped and 8-bit layers read them."""
+        units = self.embed_layer.output_units
+        batch = offsets[0].numel() - int(include_last_offset)
+        per = 16 // self.embed_layer.output_dtype.itemsize
+        if units % per == 0 or batch < 0:
+            return self.embed_layer(values, offsets, include_last_offset=include_last_offset)
+        out = torch.empty((batch, (units + per - 1) // per * per), dtype=self.embed_layer.output_dtype, device=self.device)
+        return self.embed_layer(values, offsets, include_last_offset=include_last_offset, out=out)[:, :units]
+
     def forward(self, values: Sequence[torch.Tensor], offsets: Sequence[torch.Tensor],
-                include_last_offset: bool = True):
-        embed_output = self.embed_layer(values, offsets, include_last_offset=include_last_offset)
-        return self.mlp(embed_output)
+                include_last_offset: bool = True, experts: Optional[torch.Tensor] = None):
+        if not self.num_experts:
+            if experts is not None:
+                raise ValueError("this model has no experts")
+            if isinstance(self.mlp[0], Int8Linear):
+                return self.mlp(self._embed(values, offsets, include_last_offset))
+            embed_output = self.embed_layer(values, offsets, include_last_offset=include_last_offset)
+            return self.mlp(embed_output)
+        rows = self._embed(values, offsets, include_last_offset)
+        if experts is None or experts.numel() != rows.shape[0]:
+            raise ValueError(f"experts must hold one expert number for each of the {rows.shape[0]} samples")
+        order, ends = group_rows(experts, self.num_experts)
+        last = len(self.mlp) - 1
+        for i, layer in enumerate(self.mlp):
+            rows = layer(rows, ends, in_rows=order if i == 0 else None, out_rows=order if i == last else None)
+        return rows
