@@ -69,6 +69,7 @@ def _units():
         ("eb_longbag.o", "eb_longbag_inst.cu", []),
         ("eb_rows.o", "eb_rows.cu", []),
         ("eb_linear.o", "eb_linear.cu", []),
+        ("eb_linear_few.o", "eb_linear_few.cu", []),
     ]
     for occ in range(1, 9):
         units.append((f"eb_fused_occ{occ}.o", "eb_fused_inst.cu", [f"-DEB_OCC={occ}"]))

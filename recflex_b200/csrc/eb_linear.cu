@@ -15,9 +15,10 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/recflex_b200.h"
-#include "eb_linear.h"
+#include "eb_linear.cuh"
 #include "eb_mma.cuh"
 
 namespace ebk {
@@ -26,24 +27,33 @@ namespace {
 using namespace mma;
 
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;  // warp 0 copies, warp 1 multiplies, the others store
+constexpr int kCopyWarps = 7;
+constexpr int kBoxWarps = 4;                           // that copy rows in order; rows by index take all of them
+constexpr int kFirstEpilogue = 32 * (kCopyWarps + 1);  // then one warp multiplies and the others store
+constexpr int kThreads = kFirstEpilogue + 32 * kEpilogueWarps;
 constexpr int kKBytes = 128;                        // K of one stage: a row of the 128-byte swizzle
 constexpr int kABytes = 128 * kKBytes;
 constexpr int kBoxRows = 32;                        // rows of x per tensor copy: a ragged tile copies only its own boxes
-constexpr int kStagingBytes = 4096;                 // per storing warp: 32 rows of 128 bytes
-constexpr int kColumnBytes = 512;                   // per storing warp: scale and bias of 64 columns
+constexpr int kColumnBytes = 1024;                  // per storing warp: scale and bias of its 128 columns
 constexpr int kSmemMax = 232448;
+constexpr int kMaxSplit = 8;                        // pieces of K: CTAs of the largest portable cluster
 
 template <int BN, int CG>
 struct Shape {
   static constexpr int kRows = 128 * CG;
-  static constexpr int kBRows = BN / CG;  // rows of the weight that one CTA of the pair copies
-  static constexpr int kStageBytes = kABytes + kBRows * kKBytes;
-  static constexpr int kFixed = 1024 /* alignment */ + kEpilogueWarps * (kStagingBytes + kColumnBytes) + 256 /* barriers */ +
+  // A tile of 512 columns is two products of 256 that share the rows of x, and takes all of tensor memory; narrower ones
+  // have two accumulators, so that one is stored while the next tile is summed.
+  static constexpr int kParts = BN > 256 ? 2 : 1;
+  static constexpr int kPart = BN / kParts;
+  static constexpr int kWRows = kPart / CG;  // rows of the weight that one CTA of a pair copies for a part
+  static constexpr int kStageBytes = kABytes + kParts * kWRows * kKBytes;
+  static constexpr int kStagingRow = kParts > 1 ? 64 : 128;  // bytes of a result row that are stored at once
+  static constexpr int kStaging = 32 * kStagingRow;          // per storing warp
+  static constexpr int kFixed = 1024 /* alignment */ + kEpilogueWarps * (kStaging + kColumnBytes) + 256 /* barriers */ +
                                 2 * 4 * (EB_MAX_GROUPS + 1) + 8;
   static constexpr int kStages = (kSmemMax - kFixed) / kStageBytes > 10 ? 10 : (kSmemMax - kFixed) / kStageBytes;
   static constexpr int kSmem = kFixed + kStages * kStageBytes;
-  static constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;  // of tensor memory: two accumulators
+  static constexpr int kCols = 2 * kPart < 32 ? 32 : 2 * kPart;  // of tensor memory
 };
 
 struct LinearArgs {
@@ -57,84 +67,44 @@ struct Tile {
   int group, m0, m1, n0;  // positions [m0, min(m1, m0 + rows)), columns from n0
 };
 
-// Offsets made non-decreasing inside [0, positions], and the number of row tiles in front of each group.  Called by
-// one whole warp.
-__device__ __forceinline__ void load_groups(const eb_linear_args& a, int* off, int* tiles, int tile_rows, uint32_t* bad) {
-  const int lane = threadIdx.x % 32;
-  const int P = (int)a.positions;
-  int high = 0, sum = 0;
-  bool wrong = false;
-  for (int base = 0; base <= a.num_groups; base += 32) {
-    const int e = base + lane;
-    const int raw = e > a.num_groups ? high : a.offsets ? a.offsets[e] : (e == 0 ? 0 : P);
-    int v = min(max(raw, 0), P);
-    wrong |= v != raw;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v = max(v, o);
-    }
-    v = max(v, high);
-    wrong |= e <= a.num_groups && v != raw;
-    int before = __shfl_up_sync(0xffffffffu, v, 1);
-    if (lane == 0) before = high;
-    const int count = e == 0 || e > a.num_groups ? 0 : v - before;
-    int t = (count + tile_rows - 1) / tile_rows;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, t, d);
-      if (lane >= d) t += o;
-    }
-    if (e <= a.num_groups) {
-      off[e] = v;
-      tiles[e] = sum + t;
-    }
-    sum += __shfl_sync(0xffffffffu, t, 31);
-    high = __shfl_sync(0xffffffffu, v, 31);
+// Two values rounded to 16 bits, each at least `low` (two of the same type); NaN stays NaN
+template <int OUT>
+__device__ __forceinline__ uint32_t pack2(float2 v, uint32_t low) {
+  uint32_t r;
+  if constexpr (OUT == EB_OUT_BF16) {
+    const __nv_bfloat162 w = __floats2bfloat162_rn(v.x, v.y);
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(*reinterpret_cast<const uint32_t*>(&w)), "r"(low));
+  } else {
+    const __half2 w = __floats2half2_rn(v.x, v.y);
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(*reinterpret_cast<const uint32_t*>(&w)), "r"(low));
   }
-  if (__any_sync(0xffffffffu, wrong) && lane == 0 && bad) atomicOr(bad, kLinearBadOffsets);
+  return r;
 }
 
-// The group whose row tiles hold tile t: the last g with tiles[g] <= t.
-__device__ __forceinline__ int find_group(const int* tiles, int num_groups, int t) {
-  int lo = 0, hi = num_groups - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (tiles[mid] <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+// Pairs of fp32 operations in one instruction, each rounded as the single one is
+__device__ __forceinline__ unsigned long long both(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 apart(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return apart(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return apart(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(both(a)), "l"(both(b)), "l"(both(c)));
+  return apart(r);
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == EB_ACT_RELU) return v < 0.0f ? 0.0f : v;  // keeps NaN
-  if (act == EB_ACT_SIGMOID) return 1.0f / (1.0f + expf(-v));
-  return v;
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
-  if (bf16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ void store_value(void* out, int64_t at, int out_dtype, float v) {
-  if (out_dtype == EB_OUT_F32)
-    static_cast<float*>(out)[at] = v;
-  else if (out_dtype == EB_OUT_BF16)
-    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else
-    static_cast<__half*>(out)[at] = __float2half_rn(v);
-}
-
+// The staging rows and partial sums are read and written by these alone, and barriers stand between the two: they need
+// no order with other memory, and loads of scales and stores of results may move past them.
 __device__ __forceinline__ uint4 shared_read(uint32_t at) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
 }
 __device__ __forceinline__ uint4 cluster_read(uint32_t at) {
@@ -143,73 +113,98 @@ __device__ __forceinline__ uint4 cluster_read(uint32_t at) {
   return v;
 }
 __device__ __forceinline__ void shared_write(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d));
 }
 
-template <bool I8>
-__device__ __forceinline__ float as_sum(uint32_t bits) {
-  if constexpr (I8) return (float)(int)bits;
-  return __uint_as_float(bits);
-}
-
-// What a position's row needs: where its result goes (-1: nowhere) and its factor (0 for a row number outside x, whose
-// products count as zeros).
-struct RowInfo {
-  int dst;
-  float scale;
-  bool zero;
-};
-
-template <bool I8>
-__device__ __forceinline__ RowInfo row_info(const eb_linear_args& a, int p, int m1) {
-  RowInfo r{-1, 1.0f, false};
-  if (p >= m1) return r;
-  const int s = a.in_rows ? __ldg(a.in_rows + p) : p;
-  const int d = a.out_rows ? __ldg(a.out_rows + p) : p;
-  uint32_t bad = 0;
-  if (s < 0 || s >= a.x_rows) {
-    r.zero = true;
-    bad |= kLinearBadInRow;
-  } else if constexpr (I8) {
-    r.scale = __ldg(a.x_scale + s);
+// SPAN columns from `n` of one accumulator row per lane (tensor memory from `tm` on), finished and stored.  A unit of
+// columns that fills a staging row goes through shared memory, so that neighbouring lanes store neighbouring 16 bytes
+// of a row wherever it goes; the 16-byte pieces of a staging row are swizzled by the row, free of bank conflicts both
+// ways.  relu is a maximum with a bound of 0 or -infinity.  What this costs is instructions (two warps share a scheduler,
+// 64 columns each at a time): 14 a value, with a bound and a branch for each, took 2000 clocks per 64 columns; pairs of
+// fp32 operations, the bound on packed pairs and a path of its own for the sigmoid leave about 5.
+template <bool I8, int OUT, bool SIGMOID, int SPAN, int ROWB>
+__device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, const RowInfo& r, const float* scales,
+                                           const float* biases, int n, uint32_t mine, int lane) {
+  const eb_linear_args& a = args.a;
+  constexpr int kSize = OUT == EB_OUT_F32 ? 4 : 2, kElems = 16 / kSize;
+  constexpr int kUnit = SPAN < ROWB / kSize ? SPAN : ROWB / kSize, kLoad = kUnit < 32 ? kUnit : 32;
+  constexpr int kPieces = kUnit / kElems, kRowsOnce = 32 / kPieces;
+  auto place = [](int row, int piece) {
+    return row * ROWB + ((ROWB == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4);
+  };
+  const float low = a.activation == EB_ACT_RELU ? 0.0f : __int_as_float(0xff800000);
+  const uint32_t low2 = a.activation == EB_ACT_RELU ? 0u : OUT == EB_OUT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+  const bool any_zero = !I8 && __any_sync(0xffffffffu, r.zero);
+  const float2 row_scale = make_float2(r.scale, r.scale);
+  const int piece = lane % kPieces;
+  uint8_t* to[kPieces];  // this lane's rows
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int dst = __shfl_sync(0xffffffffu, r.dst, i * kRowsOnce + lane / kPieces);
+    to[i] = dst < 0 ? nullptr : static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + n) * kSize + piece * 16;
   }
-  if (d < 0 || d >= a.out_rows_total)
-    bad |= kLinearBadOutRow;
-  else
-    r.dst = d;
-  if (bad) atomicOr(a.status, bad);
-  return r;
-}
-
-// One result: in fp32, scaled by the row's and the column's factor, plus the bias.
-template <bool I8>
-__device__ __forceinline__ float finish(uint32_t bits, const RowInfo& r, float col_scale, float bias, int act) {
-  float v = r.zero ? 0.0f : as_sum<I8>(bits);
-  if constexpr (I8)
-    v = __fmaf_rn(v, __fmul_rn(r.zero ? 0.0f : r.scale, col_scale), bias);
-  else
-    v += bias;
-  return activate(v, act);
-}
-
-// N columns from `col` of one accumulator row per lane, finished, into `words` (16-bit types two to a word).
-template <bool I8, int N>
-__device__ __forceinline__ void finish_columns(const uint32_t (&v)[N], const RowInfo& r, const float* scales,
-                                               const float* biases, const eb_linear_args& a, uint32_t at, int piece0,
-                                               int lane) {
-  const bool f32 = a.out_dtype == EB_OUT_F32, bf16 = a.out_dtype == EB_OUT_BF16;
+#pragma unroll 1
+  for (int c = 0; c < SPAN && n + c < a.n; c += kUnit) {
+    uint32_t v[kUnit];
 #pragma unroll
-  for (int i = 0; i < N; i += 8) {
-    float o[8];
+    for (int i = 0; i < kUnit; i += kLoad) tmem_load(tm + c + i, *reinterpret_cast<uint32_t(*)[kLoad]>(v + i));
+    tmem_wait_load();
+    __syncwarp();  // the unit before has been read
+    if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = finish<I8>(v[i + j], r, I8 ? scales[i + j] : 1.0f, biases[i + j], a.activation);
-    if (f32) {
-      const int p0 = piece0 + i / 4;
-      shared_write(at + ((p0 ^ (lane & 7)) << 4), __float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
-      shared_write(at + (((p0 + 1) ^ (lane & 7)) << 4), __float_as_uint(o[4]), __float_as_uint(o[5]), __float_as_uint(o[6]), __float_as_uint(o[7]));
-    } else {
-      const int p0 = piece0 + i / 8;
-      shared_write(at + ((p0 ^ (lane & 7)) << 4), pack2(o[0], o[1], bf16), pack2(o[2], o[3], bf16), pack2(o[4], o[5], bf16), pack2(o[6], o[7], bf16));
+      for (int i = 0; i < kUnit; ++i) v[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnit; i += 8) {
+      float2 o[4], f[4], b[4];
+      *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(biases + c + i);
+      *reinterpret_cast<float4*>(b + 2) = *reinterpret_cast<const float4*>(biases + c + i + 4);
+      if constexpr (I8) {  // a row number outside x has a factor of 0
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(scales + c + i);
+        *reinterpret_cast<float4*>(f + 2) = *reinterpret_cast<const float4*>(scales + c + i + 4);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = v[i + 2 * j], y = v[i + 2 * j + 1];
+        if constexpr (I8)
+          o[j] = fma2(make_float2((float)(int)x, (float)(int)y), mul2(row_scale, f[j]), b[j]);
+        else
+          o[j] = add2(make_float2(__uint_as_float(x), __uint_as_float(y)), b[j]);
+        if constexpr (SIGMOID) o[j] = make_float2(sigmoid(o[j].x), sigmoid(o[j].y));
+        if constexpr (OUT == EB_OUT_F32) o[j] = make_float2(at_least(o[j].x, low), at_least(o[j].y, low));
+      }
+      if constexpr (OUT == EB_OUT_F32) {
+        shared_write(mine + place(lane, i / 4), __float_as_uint(o[0].x), __float_as_uint(o[0].y), __float_as_uint(o[1].x), __float_as_uint(o[1].y));
+        shared_write(mine + place(lane, i / 4 + 1), __float_as_uint(o[2].x), __float_as_uint(o[2].y), __float_as_uint(o[3].x), __float_as_uint(o[3].y));
+      } else {
+        shared_write(mine + place(lane, i / 8), pack2<OUT>(o[0], low2), pack2<OUT>(o[1], low2), pack2<OUT>(o[2], low2), pack2<OUT>(o[3], low2));
+      }
+    }
+    __syncwarp();
+    const bool whole = args.wide && n + c + kUnit <= a.n;
+    uint4 out[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) out[i] = shared_read(mine + place(i * kRowsOnce + lane / kPieces, piece));
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint4 w = out[i];
+      uint8_t* at = to[i] + c * kSize;
+      if (!to[i]) continue;
+      if (whole) {
+        *reinterpret_cast<uint4*>(at) = w;
+        continue;
+      }
+      const int left = a.n - (n + c + piece * kElems);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < kElems; ++j) {
+        if (j < left) {
+          if constexpr (kSize == 4)
+            reinterpret_cast<uint32_t*>(at)[j] = words[j];
+          else
+            reinterpret_cast<uint16_t*>(at)[j] = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
+        }
+      }
     }
   }
 }
@@ -221,6 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     eb_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_w) {
   using S = Shape<BN, CG>;
+  static_assert(kBoxRows * kBoxWarps == 128 && (CG == 1 || CG == 2), "rows of a CTA");
   static_assert(!SPLIT || CG == 1, "a pair of CTAs shares its tile already");
   constexpr int kStages = S::kStages;
   constexpr int kStep = I8 ? kKBytes : kKBytes / 2;  // elements of K per stage
@@ -229,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
   uint8_t* base = smem_raw + (ring - smem_addr(smem_raw));
   const uint32_t staging = ring + kStages * S::kStageBytes;
-  uint8_t* after = base + kStages * S::kStageBytes + kEpilogueWarps * kStagingBytes;
+  uint8_t* after = base + kStages * S::kStageBytes + kEpilogueWarps * S::kStaging;
   float* columns = reinterpret_cast<float*>(after);
   after += kEpilogueWarps * kColumnBytes;
   const uint32_t bars = smem_addr(after);
@@ -249,8 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_map(&map_x);
       prefetch_map(&map_w);
     }
-    load_groups(a, off, tiles, S::kRows, blockIdx.x == 0 ? a.status : nullptr);
-  } else if (warp == 1) {
+    groups_of(a, off, tiles, S::kRows, blockIdx.x == 0 ? a.status : nullptr);
+  } else if (warp == kCopyWarps) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
         bar_init(full + 8 * i, 1);
@@ -295,43 +291,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     return a.in_rows ? (rows + 3) / 4 * 4 * kKBytes : (rows + kBoxRows - 1) / kBoxRows * kBoxRows * kKBytes;
   };
 
-  uint32_t copied = 0;  // stages filled so far (warp 0)
-  if (warp == 0) {
+  uint32_t copied = 0;  // stages filled so far (copying warps)
+  if (warp < kCopyWarps) {
     bool ok = true;
+    const bool idle = !a.in_rows && warp >= kBoxWarps;
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride) {
       const Tile tile = tile_at(t);
       const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
       const int rows = rows_of(tile, rank);
-      uint32_t bytes = bytes_of(tile, 0) + CG * S::kBRows * kKBytes;
+      uint32_t bytes = bytes_of(tile, 0) + CG * S::kParts * S::kWRows * kKBytes;
       if constexpr (CG > 1) bytes += bytes_of(tile, 1);
+      // the copying warps share the rows: by index four at a time (a lane each), in order one box of 32 each.  (A warp's
+      // lanes issue their copies one after the other: by index, 4 warps took 639 us for 16384 x 15608 x 1024 in bf16 where
+      // 8 took 542 us, both on 256 x 256 tiles.  7 leave the other warps 128 registers.)
+      const int quad = lane * kCopyWarps + warp;
+      const bool copies = a.in_rows ? 4 * quad < rows : lane == 0 && kBoxRows * warp < rows;
       int4 src = make_int4(0, 0, 0, 0);  // rows that do not exist read row 0: their products are not used
-      if (a.in_rows) {
+      if (a.in_rows && copies) {
         int* s = reinterpret_cast<int*>(&src);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int i = 4 * lane + j;
+          const int i = 4 * quad + j;
           if (i < rows) {
             const int r = __ldg(a.in_rows + m_cta + i);
             s[j] = r >= 0 && r < a.x_rows ? r : 0;
           }
         }
       }
-      for (int k = k_first; k < k_last && ok; ++k) {
+      for (int k = k_first; k < k_last && ok && !idle; ++k) {
         const uint32_t st = copied % kStages, phase = (copied / kStages) & 1;
         ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * st, phase ^ 1, gave_up));
         if (!ok) break;
         const uint32_t sx = ring + st * S::kStageBytes, sw = sx + kABytes;
         uint32_t bar = full + 8 * st;
-        if (leader) {
-          if (lane == 0) bar_expect(bar, bytes);
-          __syncwarp();
-        }
+        if (leader && threadIdx.x == 0) bar_expect(bar, bytes);
         if constexpr (CG > 1) bar = map_rank(bar, 0);
-        if (lane == 0) load_3d<CG>(sw, &map_w, k * kStep, tile.n0 + (CG > 1 ? S::kBRows * (int)rank : 0), tile.group, bar);
-        if (a.in_rows) {
-          if (4 * lane < rows) load_rows4<CG>(sx + lane * 4 * kKBytes, &map_x, k * kStep, src, bar);
-        } else {
-          if (kBoxRows * lane < rows) load_2d<CG>(sx + lane * kBoxRows * kKBytes, &map_x, k * kStep, m_cta + kBoxRows * lane, bar);
+        if (warp < S::kParts && lane == 0)
+          load_3d<CG>(sw + warp * S::kWRows * kKBytes, &map_w, k * kStep, tile.n0 + warp * S::kPart + (CG > 1 ? S::kWRows * (int)rank : 0), tile.group, bar);
+        if (copies) {
+          if (a.in_rows)
+            load_rows4<CG>(sx + quad * 4 * kKBytes, &map_x, k * kStep, src, bar);
+          else
+            load_2d<CG>(sx + warp * kBoxRows * kKBytes, &map_x, k * kStep, m_cta + kBoxRows * warp, bar);
         }
         ++copied;
       }
@@ -341,28 +342,62 @@ __global__ void __launch_bounds__(kThreads, 1)
         cluster_sync();
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == kCopyWarps) {
     bool ok = true;
     uint32_t used = 0, count = 0;
-    const uint32_t desc = product_of(I8, a.dtype == EB_OUT_BF16, S::kRows, BN);
+    const uint32_t desc = product_of(I8, a.dtype == EB_OUT_BF16, S::kRows, S::kPart);
+    auto wait_full = [&](uint32_t at) {
+      const bool there = bar_wait(full + 8 * (at % kStages), (at / kStages) & 1, gave_up);
+      fence_after();
+      return there;
+    };
+    auto wait_drained = [&](uint32_t slot, uint32_t turn) {
+      const bool there = bar_wait(drained + 8 * slot, (turn & 1) ^ 1, gave_up);
+      fence_after();
+      return there;
+    };
+    auto products = [&](uint32_t at, uint32_t slot, int part, bool add) {
+      const uint32_t x = ring + (at % kStages) * S::kStageBytes;
+      const uint64_t ax = operand(x), bw = operand(x + kABytes + part * S::kWRows * kKBytes);
+#pragma unroll
+      for (int i = 0; i < kKBytes / 32; ++i) multiply<I8, CG>(tmem + slot * S::kPart, ax + 2 * i, bw + 2 * i, desc, add || i > 0);
+    };
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride, ++count) {
       if (leader && lane == 0) {
-        const uint32_t acc = count & 1;
-        const uint32_t d = tmem + acc * BN;
-        ok = ok && bar_wait(drained + 8 * acc, ((count >> 1) & 1) ^ 1, gave_up);
-        fence_after();
-        for (int k = k_first; k < k_last && ok; ++k, ++used) {
-          const uint32_t st = used % kStages, phase = (used / kStages) & 1;
-          ok = bar_wait(full + 8 * st, phase, gave_up);
-          if (!ok) break;
-          fence_after();
-          const uint64_t ax = operand(ring + st * S::kStageBytes), bw = operand(ring + st * S::kStageBytes + kABytes);
-#pragma unroll
-          for (int i = 0; i < kKBytes / 32; ++i)
-            multiply<I8, CG>(d, ax + 2 * i, bw + 2 * i, desc, k > k_first || i > 0);
-          commit<CG>(empty + 8 * st);
+        const int steps = k_last - k_first;
+        if constexpr (S::kParts == 1) {
+          const uint32_t slot = count & 1;
+          ok = ok && wait_drained(slot, count >> 1);
+          for (int k = 0; k < steps && ok; ++k, ++used) {
+            ok = wait_full(used);
+            if (!ok) break;
+            products(used, slot, 0, k > 0);
+            commit<CG>(empty + 8 * (used % kStages));
+          }
+          if (ok) commit<CG>(done + 8 * slot);
+        } else {
+          // the first stages' products with the first 256 columns run while the second 256 of the tile before are stored
+          const int early = steps < kStages ? steps : kStages;
+          ok = ok && wait_drained(0, count);
+          for (int k = 0; k < early && ok; ++k) {
+            ok = wait_full(used + k);
+            if (ok) products(used + k, 0, 0, k > 0);
+          }
+          ok = ok && wait_drained(1, count);
+          for (int k = 0; k < steps && ok; ++k, ++used) {
+            if (k >= early) {
+              ok = wait_full(used);
+              if (!ok) break;
+              products(used, 0, 0, true);
+            }
+            products(used, 1, 1, k > 0);
+            commit<CG>(empty + 8 * (used % kStages));
+          }
+          if (ok) {
+            commit<CG>(done);
+            commit<CG>(done + 8);
+          }
         }
-        if (ok) commit<CG>(done + 8 * acc);
       }
       if constexpr (SPLIT) {
         __syncwarp();
@@ -377,96 +412,103 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_wait(last, 0, &keep);
     }
   } else {
-    const int e = warp - 2, quad = warp % 4, half = e / 4;
-    const uint32_t mine = staging + e * kStagingBytes;
+    const int e = warp - kCopyWarps - 1, quad = warp % 4, half = e / 4;
+    const uint32_t mine = staging + e * S::kStaging;
     float* col_scale = columns + e * (kColumnBytes / 4);
-    float* col_bias = col_scale + 64;
-    const int size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
-    if (a.zero_rest) {
-      const int64_t group_rows = off[a.num_groups] - off[0];
-      const int64_t rest = (a.positions - group_rows) * a.n;
-      for (int64_t i = (int64_t)blockIdx.x * (32 * kEpilogueWarps) + threadIdx.x - 64; i < rest;
-           i += (int64_t)gridDim.x * (32 * kEpilogueWarps)) {
-        int64_t p = i / a.n;
-        if (p >= off[0]) p += group_rows;
-        const int64_t d = a.out_rows ? a.out_rows[p] : p;
-        if (d >= 0 && d < a.out_rows_total) store_value(a.out, d * a.out_ld + i % a.n, a.out_dtype, 0.0f);
+    float* col_bias = col_scale + 128;
+    if (a.zero_rest)
+      zero_rest(a, off, (int64_t)blockIdx.x * (32 * kEpilogueWarps) + threadIdx.x - kFirstEpilogue,
+                (int64_t)gridDim.x * (32 * kEpilogueWarps));
+    // what the next tile needs besides its products: this lane's row, and the scales and biases of its columns
+    constexpr int kColumnsEach = S::kPart >= 64 ? S::kPart / 64 : 1;
+    RowInfo next_row{-1, 0.0f, false};
+    float next_scale[kColumnsEach], next_bias[kColumnsEach];
+    auto fetch_row = [&](int64_t t) {
+      const Tile tile = tile_at(t);
+      const int p = tile.m0 + (CG > 1 ? 128 * (int)rank : 0) + quad * 32 + lane;
+      next_row = row_info<I8>(a, p, S::kPart >= 64 || half == 0 ? tile.m1 : 0);
+    };
+    auto fetch_columns = [&](int64_t t, int part) {
+      const Tile tile = tile_at(t);
+      const int n = tile.n0 + part * S::kPart + (S::kPart >= 64 ? half * (S::kPart / 2) : 0) + lane;
+      const int64_t at = (int64_t)tile.group * a.n + n;
+#pragma unroll
+      for (int i = 0; i < kColumnsEach; ++i) {
+        const bool in = n + 32 * i < a.n;
+        next_scale[i] = I8 && in ? __ldg(a.w_scale + at + 32 * i) : 0.0f;
+        next_bias[i] = in && a.bias ? __ldg(a.bias + at + 32 * i) : 0.0f;
       }
-    }
+    };
     bool ok = true;
     uint32_t count = 0;
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride, ++count) {
       const Tile tile = tile_at(t);
-      const uint32_t acc = count & 1;
       const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
       const int rows = rows_of(tile, rank);
-      const uint32_t d = tmem + acc * BN + ((uint32_t)(quad * 32) << 16);
       if constexpr (!SPLIT) {
-        constexpr int kHalves = BN >= 64 ? 2 : 1;  // narrow tiles: one warp takes all columns of its lanes
-        constexpr int kSpan = BN / kHalves;
-        constexpr int kLoad = kSpan < 32 ? kSpan : 32;
+        constexpr int kHalves = S::kPart >= 64 ? 2 : 1;  // narrow tiles: one warp takes all columns of its lanes
+        constexpr int kSpan = S::kPart / kHalves;
+        constexpr int kEach = (kSpan + 31) / 32;
         const bool work = half < kHalves && quad * 32 < rows;
-        RowInfo r{-1, 1.0f, false};
-        if (work) r = row_info<I8>(a, m_cta + quad * 32 + lane, tile.m1);
-        ok = __all_sync(0xffffffffu, bar_wait(done + 8 * acc, (count >> 1) & 1, gave_up));
-        if (!ok) break;
-        fence_after();
-        if (work) {
-          const int unit = size == 4 ? kLoad : (kSpan < 64 ? kSpan : 64);  // columns that go through the staging rows at once
-          for (int c = half * kSpan; c < (half + 1) * kSpan && tile.n0 + c < a.n; c += unit) {
-            const int n = tile.n0 + c;
-            __syncwarp();
-            for (int i = lane; i < unit; i += 32) {
-              const bool in = n + i < a.n;
-              const int64_t at = (int64_t)tile.group * a.n + n + i;
-              if constexpr (I8) col_scale[i] = in ? __ldg(a.w_scale + at) : 0.0f;
-              col_bias[i] = in && a.bias ? __ldg(a.bias + at) : 0.0f;
-            }
-            __syncwarp();
-            for (int u = 0; u < unit; u += kLoad) {
-              uint32_t v[kLoad];
-              tmem_load(d + c + u, v);
-              tmem_wait_load();
-              finish_columns<I8, kLoad>(v, r, col_scale + u, col_bias + u, a, mine + lane * 128, u * size / 16, lane);
-            }
-            __syncwarp();
-            const int per_row = unit * size / 16, elems = 16 / size;  // pieces of 16 bytes, values in a piece
-            const int rows_once = 32 / per_row;
-            for (int i = 0; i < per_row; ++i) {
-              const int row = i * rows_once + lane / per_row, piece = lane % per_row;
-              const int dst = __shfl_sync(0xffffffffu, r.dst, row);
-              const int col = n + piece * elems;
-              if (dst < 0 || col >= a.n) continue;
-              const uint4 w = shared_read(mine + row * 128 + ((piece ^ (row & 7)) << 4));
-              uint8_t* to = static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + col) * size;
-              if (args.wide && col + elems <= a.n) {
-                *reinterpret_cast<uint4*>(to) = w;
-                continue;
-              }
-              const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-              if (size == 4) {
+        if (count == 0) {
+          fetch_row(t);
+          fetch_columns(t, 0);
+        }
+        const RowInfo r = next_row;
+#pragma unroll 1
+        for (int part = 0; part < S::kParts; ++part) {
+          const uint32_t slot = S::kParts > 1 ? part : count & 1, turn = S::kParts > 1 ? count : count >> 1;
+          const int n = tile.n0 + part * S::kPart + half * kSpan;
+          __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (col + j < a.n) reinterpret_cast<uint32_t*>(to)[j] = words[j];
-              } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (col + j < a.n) reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
-              }
+          for (int i = 0; i < kEach; ++i) {
+            if (32 * i + lane < kSpan) {
+              if constexpr (I8) col_scale[32 * i + lane] = next_scale[i];
+              col_bias[32 * i + lane] = next_bias[i];
             }
           }
-        }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG > 1)
-            bar_arrive_cluster(map_rank(drained + 8 * acc, 0));
-          else
-            bar_arrive(drained + 8 * acc);
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, bar_wait(done + 8 * slot, turn & 1, gave_up));
+          if (!ok) break;
+          fence_after();
+          // on their way while this part is stored
+          if (part + 1 < S::kParts) {
+            fetch_columns(t, part + 1);
+          } else if (t + stride < total) {
+            fetch_row(t + stride);
+            fetch_columns(t + stride, 0);
+          }
+          if (work) {
+            const uint32_t tm = tmem + slot * S::kPart + half * kSpan + ((uint32_t)(quad * 32) << 16);
+            auto store = [&](auto out, auto sigmoid) {
+              store_span<I8, decltype(out)::value, decltype(sigmoid)::value, kSpan, S::kStagingRow>(args, tm, r, col_scale, col_bias, n, mine, lane);
+            };
+            auto store_as = [&](auto out) {
+              if (a.activation == EB_ACT_SIGMOID)
+                store(out, std::true_type{});
+              else
+                store(out, std::false_type{});
+            };
+            if (a.out_dtype == EB_OUT_BF16)
+              store_as(std::integral_constant<int, EB_OUT_BF16>{});
+            else if (a.out_dtype == EB_OUT_F16)
+              store_as(std::integral_constant<int, EB_OUT_F16>{});
+            else if constexpr (I8)
+              store_as(std::integral_constant<int, EB_OUT_F32>{});
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG > 1)
+              bar_arrive_cluster(map_rank(drained + 8 * slot, 0));
+            else
+              bar_arrive(drained + 8 * slot);
+          }
         }
       } else {
         // every CTA lays its partial sums out in its ring (all its copies and products are done)
         constexpr int kPieces = BN / 4;  // of 16 bytes in a row
+        const uint32_t acc = count & 1, d = tmem + acc * BN + ((uint32_t)(quad * 32) << 16);
         ok = ok && __all_sync(0xffffffffu, bar_wait(done + 8 * acc, (count >> 1) & 1, gave_up));
         fence_after();
         if (ok && quad * 32 < rows) {
@@ -486,24 +528,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         cluster_sync();
         if (ok) {
-          const int id = (threadIdx.x - 64) * pieces + rank;
+          const int id = (threadIdx.x - kFirstEpilogue) * pieces + rank;
           for (int i = id; i < rows * kPieces; i += 32 * kEpilogueWarps * pieces) {
             const int row = i / kPieces, piece = i % kPieces, n = tile.n0 + piece * 4;
             if (n >= a.n) continue;
             const uint32_t at = ring + row * (BN * 4) + ((piece ^ (row & 7)) << 4);
+            const RowInfo r = row_info<I8>(a, m_cta + row, tile.m1);
             uint32_t sum[4] = {};
-            for (int s = 0; s < pieces; ++s) {
-              const uint4 w = cluster_read(map_rank(at, s));
-              const uint32_t p[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if constexpr (I8)
-                  sum[j] += p[j];
-                else
-                  sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(p[j]));
+            for (int s0 = 0; s0 < kMaxSplit; s0 += 4) {  // four reads at a time on their way
+              uint4 part[4];
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                if (s0 + s < pieces) part[s] = cluster_read(map_rank(at, s0 + s));
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                if (s0 + s >= pieces) break;
+                const uint32_t p[4] = {part[s].x, part[s].y, part[s].z, part[s].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  sum[j] = I8 ? sum[j] + p[j] : __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(p[j]));
               }
             }
-            const RowInfo r = row_info<I8>(a, m_cta + row, tile.m1);
             if (r.dst < 0) continue;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -537,10 +583,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if constexpr (CG > 1 || SPLIT) cluster_sync();
+  if constexpr (CG > 1 || SPLIT) cluster_meet();
   fence_after();
   __syncwarp();
-  if (warp == 1) tmem_free<CG>(tmem, S::kCols);
+  if (warp == kCopyWarps) tmem_free<CG>(tmem, S::kCols);
 }
 
 // ---- host ------------------------------------------------------------------
@@ -578,7 +624,6 @@ bool make_map(CUtensorMap* map, int dims, int dtype, const void* p, int64_t k, i
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxRows = 0x7fffffffLL - 1024;  // row numbers of a whole tile behind the last row still fit 32 bits
 
 template <bool I8, int BN, int CG, bool SPLIT>
@@ -591,7 +636,7 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   // rows of x that are all out of range are never used: any memory of the right length will do
   const void* x = a.x_rows ? a.x : a.weight;
   if (!make_map(&map_x, 2, a.dtype, x, a.k, a.x_rows ? a.x_rows : 1, a.x_ld, 1, 0, a.in_rows ? 1 : kBoxRows) ||
-      !make_map(&map_w, 3, a.dtype, a.weight, a.k, a.n, a.w_ld, a.num_groups, a.w_group_ld, S::kBRows))
+      !make_map(&map_w, 3, a.dtype, a.weight, a.k, a.n, a.w_ld, a.num_groups, a.w_group_ld, S::kWRows))
     return linear_fail(EB_ERR_INVALID_ARG, "the driver refused a tensor map for %d x %d of pitch %lld / %lld", a.n, a.k,
                        (long long)a.x_ld, (long long)a.w_ld);
   const auto kernel = eb_linear_kernel<I8, BN, CG, SPLIT>;
@@ -619,19 +664,6 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   return EB_OK;
 }
 
-int sm_count(int device) {
-  static std::atomic<int> known[kMaxDevices];
-  int n = known[device].load();
-  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess) known[device].store(n);
-  return n;
-}
-
-// Row tiles of `rows` rows at most: every group may end inside one.
-int64_t row_tiles(const eb_linear_args& a, int rows) {
-  const int64_t groups = a.num_groups < a.positions ? a.num_groups : a.positions;
-  return a.num_groups == 1 ? (a.positions + rows - 1) / rows : a.positions / rows + groups;
-}
-
 template <bool I8>
 int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   const eb_linear_args& a = args.a;
@@ -639,13 +671,16 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   if (sms < 2) return linear_fail(EB_ERR_CUDA, "cannot read the SM count of device %d", device);
   args.k_steps = (int)(((int64_t)a.k * (I8 ? 1 : 2) + kKBytes - 1) / kKBytes);
   const int64_t m128 = row_tiles(a, 128), m256 = row_tiles(a, 256);
+  if (a.positions <= kFewRows) return launch_few(a, sms, st);
+  if (a.n <= kNarrow) return launch_narrow(a, sms, st);
   if (a.n <= 16) return launch<I8, 16, 1, false>(args, device, sms, m128, 1, st);
   const int64_t t64 = m128 * ((a.n + 63) / 64);
   int split = 1;
-  while (split < 8 && t64 * split * 2 <= sms && split * 2 <= args.k_steps) split *= 2;
+  while (split < kMaxSplit && t64 * split * 2 <= sms && split * 2 <= args.k_steps) split *= 2;
   if (split > 1) return launch<I8, 64, 1, true>(args, device, sms, m128, split, st);
   if (t64 <= sms || a.n <= 64) return launch<I8, 64, 1, false>(args, device, sms, m128, 1, st);
   if (a.n <= 128) return launch<I8, 128, 2, false>(args, device, sms, m256, 1, st);
+  if (a.n > 256 && args.k_steps >= 64) return launch<I8, 512, 2, false>(args, device, sms, m256, 1, st);
   return launch<I8, 256, 2, false>(args, device, sms, m256, 1, st);
 }
 
@@ -667,6 +702,7 @@ int eb_linear(const eb_linear_args* args, int device, void* stream) {
   if (a.n < 1 || a.k < 1 || a.num_groups < 1 || a.positions < 0 || a.x_rows < 0 || a.out_rows_total < 0)
     return linear_fail(EB_ERR_INVALID_ARG, "bad size: n %d, k %d, num_groups %d", a.n, a.k, a.num_groups);
   if (a.num_groups > EB_MAX_GROUPS) return linear_fail(EB_ERR_TOO_LARGE, "%d groups, at most %d", a.num_groups, EB_MAX_GROUPS);
+  if (a.k > (1 << 30)) return linear_fail(EB_ERR_TOO_LARGE, "%d columns, at most 2^30", a.k);
   if (i8 && a.k > EB_MAX_I8_COLS) return linear_fail(EB_ERR_TOO_LARGE, "%d columns of 8 bits, at most %d", a.k, EB_MAX_I8_COLS);
   if (a.positions > kMaxRows || a.x_rows > kMaxRows || a.out_rows_total > kMaxRows)
     return linear_fail(EB_ERR_TOO_LARGE, "more than %lld rows", (long long)kMaxRows);

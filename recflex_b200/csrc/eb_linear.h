@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/recflex_b200.h"
+
 namespace ebk {
 
 // Bits of the status word of eb_linear
@@ -23,6 +25,23 @@ struct DeviceScope {
     if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
   }
 };
+
+constexpr int kMaxDevices = 64;
+
+// Products of at most this many positions, and of at most this many units, run on the ordinary arithmetic units.
+constexpr int kFewRows = 8;
+constexpr int kNarrow = 4;
+int launch_few(const eb_linear_args& a, int sms, cudaStream_t st);
+int launch_narrow(const eb_linear_args& a, int sms, cudaStream_t st);
+
+// Row tiles of `rows` rows at most: every group may end inside one.
+inline int64_t row_tiles(const eb_linear_args& a, int rows) {
+  const int64_t groups = a.num_groups < a.positions ? a.num_groups : a.positions;
+  return a.num_groups == 1 ? (a.positions + rows - 1) / rows : a.positions / rows + groups;
+}
+
+// SMs of a device, 0 if that cannot be read.
+int sm_count(int device);
 
 // Sets eb_last_error() (printf style) and returns `code`.
 int linear_fail(int code, const char* fmt, ...);

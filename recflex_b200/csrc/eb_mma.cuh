@@ -25,6 +25,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// The same without ordering memory: only keeps the CTAs of a cluster alive for one another.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+
 // ---- mbarriers -------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -36,9 +41,10 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// `bar` may lie in another CTA of the cluster.
+// `bar` may lie in another CTA of the cluster.  Orders tensor memory (behind fence_before) and shared memory, not results
+// on their way to global memory: a release for the whole cluster waits until those have landed, 1400 clocks a tile.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -50,23 +56,19 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr long long kWaitLimitClocks = 4000000000ll;  // two seconds at the highest clock
 
 // Waits for the phase `parity` of a barrier; false when `gave_up` is set or the limit is reached (which sets it).
+// The clock is looked at only now and then: reading it in every wait cost more than the wait.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
   if (bar_try(bar, parity)) return true;
-  const uint64_t start = now_ns();
+  long long start = 0;
   for (uint32_t i = 1;; ++i) {
     if (bar_try(bar, parity)) return true;
-    if (i % 64 == 0) {
+    if (i % 256 == 0) {
       if (*gave_up) return false;
-      if (now_ns() - start > kWaitLimitNs) {
+      if (start == 0) start = clock64();
+      if (clock64() - start > kWaitLimitClocks) {
         *gave_up = 1;
         return false;
       }

@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -20,6 +21,14 @@ int linear_fail(int code, const char* fmt, ...) {
   va_end(ap);
   set_last_error(buf);
   return code;
+}
+
+int sm_count(int device) {
+  static std::atomic<int> known[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return 0;
+  int n = known[device].load();
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess) known[device].store(n);
+  return n;
 }
 
 namespace {
@@ -67,65 +76,109 @@ __device__ __forceinline__ void unpack(const Raw<__half>& r, float v[8]) {
   }
 }
 
+// The first `n` values of a chunk one by one, the others 0 (which changes neither a row's largest magnitude nor a code
+// that is stored).
 template <typename T>
-__device__ __forceinline__ Raw<T> load_chunk8(const T* __restrict__ row, int64_t c, int64_t cols, bool wide) {
+__device__ __forceinline__ Raw<T> load_values(const T* __restrict__ at, int n) {
   Raw<T> r;
-  constexpr int kPer = sizeof(Raw<T>) / 16;
-  uint4* dst = reinterpret_cast<uint4*>(&r);
-  const int64_t e = c * 8;
-  if (wide && e + 8 <= cols) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) dst[i] = __ldcs(reinterpret_cast<const uint4*>(row + e) + i);
-    return r;
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) dst[i] = make_uint4(0, 0, 0, 0);
   uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {  // zeros behind the row's end change neither its largest magnitude nor a stored code
-    if (e + i < cols) {
+  for (int i = 0; i < (int)sizeof(r) / 4; ++i) w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i < n) {
       if constexpr (sizeof(T) == 4)
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + e + i);
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
       else
-        w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(row) + e + i) << (16 * (i & 1));
+        w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(at) + i) << (16 * (i & 1));
     }
   }
   return r;
 }
-
-// Largest |value| of a chunk as the bits of an fp32: as integers these order infinities above every number and NaN above those.
 template <typename T>
-__device__ __forceinline__ uint32_t top_bits(const Raw<T>& r) {
-  float v[8];
-  unpack(r, v);
-  uint32_t m = 0;
+__device__ __forceinline__ Raw<T> load_wide(const T* __restrict__ at) {
+  Raw<T> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
+  for (int i = 0; i < (int)sizeof(r) / 16; ++i) reinterpret_cast<uint4*>(&r)[i] = __ldcs(reinterpret_cast<const uint4*>(at) + i);
+  return r;
+}
+
+// Running largest |value|, kept as the type is; NaN wins.  top_bits gives it as the bits of an fp32: as integers these
+// order infinities above every number and NaN above those.
+template <typename T>
+struct Top {
+  uint32_t m = 0;
+};
+__device__ __forceinline__ void widen(Top<float>& t, const Raw<float>& r) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  float m = __uint_as_float(t.m);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(__uint_as_float(w[i]))));
+  t.m = __float_as_uint(m);
+}
+__device__ __forceinline__ void widen(Top<__nv_bfloat16>& t, const Raw<__nv_bfloat16>& r) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(t.m) : "r"(w[i] & 0x7fff7fffu));
+}
+__device__ __forceinline__ void widen(Top<__half>& t, const Raw<__half>& r) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(t.m) : "r"(w[i] & 0x7fff7fffu));
+}
+__device__ __forceinline__ uint32_t top_bits(const Top<float>& t) { return t.m & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t top_bits(const Top<__nv_bfloat16>& t) {
+  return max(t.m << 16, t.m & 0x7fff0000u) & 0x7fffffffu;
+}
+__device__ __forceinline__ uint32_t top_bits(const Top<__half>& t) {
+  const float lo = __half2float(__ushort_as_half((unsigned short)(t.m & 0xffff)));
+  const float hi = __half2float(__ushort_as_half((unsigned short)(t.m >> 16)));
+  return max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu);
+}
+
+// What a row's largest magnitude makes of its codes
+struct RowScale {
+  float scale, inv, half;  // half = 0: every chunk takes the careful path
+  float up;                // power of two that the careful path multiplies by
+  bool zero;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t m) {
+  RowScale r;
+  const bool finite = m < 0x7f800000u;
+  r.scale = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(m);
+  const bool small = r.scale < 0x1p-100f;  // residuals would lose bits among the subnormals
+  r.up = small ? 0x1p100f : 1.0f;
+  r.inv = __fdiv_rn(1.0f, r.scale * r.up);
+  r.half = small ? 0.0f : 0.5f * r.scale;
+  r.zero = !finite || r.scale == 0.0f;
+  return r;
 }
 
 // Codes of 8 values.  With t = x * (1 / scale) rounded by one fused add of 1.5 * 2^23 (whose low bits then hold the
 // integer r), r is the nearest integer of the exact quotient unless that lies within a rounding error of the middle of
 // two integers.  The residual x - r * scale is exact in fp32 wherever it decides: for r = 0 it is x, for r = 1 the
 // operands are within a factor of 2, and for r >= 2 it is a multiple of scale's last place below 2^23 of them; so
-// |residual| < scale / 2 proves r, and everything else (ties among it) is divided in 64 bits, where the quotient of two
-// 24-bit significands cannot round onto a middle that it does not equal.
-__device__ __forceinline__ uint2 codes8(const float v[8], float scale, float inv, float half) {
+// |residual| < scale / 2 proves r.  The others (ties among them) take the careful path, where the same residual says
+// which neighbour is nearer.
+__device__ __forceinline__ uint2 codes8(const float v[8], const RowScale& s) {
   constexpr float kMagic = 12582912.0f;
   uint32_t b[8];
   float worst = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = __fmaf_rn(v[i], inv, kMagic);
+    const float t = __fmaf_rn(v[i], s.inv, kMagic);
     b[i] = __float_as_uint(t);
-    const float r = __fsub_rn(t, kMagic);
-    worst = fmaxf(worst, fabsf(__fmaf_rn(-r, scale, v[i])));
+    worst = fmaxf(worst, fabsf(__fmaf_rn(-__fsub_rn(t, kMagic), s.scale, v[i])));
   }
-  if (!(worst < half)) {
+  if (!(worst < s.half)) {
+    const float scale = s.scale * s.up, half = 0.5f * scale;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const double q = rint((double)v[i] / (double)scale);
-      b[i] = (uint32_t)(int)fmin(fmax(q, -127.0), 127.0);
+      const float x = v[i] * s.up;
+      float r = rintf(x * s.inv);
+      const float e = __fmaf_rn(-r, scale, x);
+      if (fabsf(e) > half || (fabsf(e) == half && ((int)r & 1))) r += copysignf(1.0f, e);
+      b[i] = (uint32_t)(int)fminf(fmaxf(r, -127.0f), 127.0f);
     }
   }
   uint2 o;
@@ -139,98 +192,144 @@ struct QuantArgs {
   int8_t* q;
   float* scale;
   int64_t rows, cols, x_ld, q_ld;
-  int wide_in, wide_out;
 };
 
-__device__ __forceinline__ void store_codes(const QuantArgs& a, int8_t* row, int64_t c, uint2 o) {
-  const int64_t e = c * 8;
-  if (e >= a.cols) return;
-  if (a.wide_out && e + 8 <= a.cols) {
-    __stcs(reinterpret_cast<uint2*>(row + e), o);
-    return;
-  }
-  for (int i = 0; i < 8 && e + i < a.cols; ++i) row[e + i] = (int8_t)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
+__device__ __forceinline__ void store_codes(int8_t* at, int n, uint2 o) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) at[i] = (int8_t)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
 }
 
 constexpr int kQuantThreads = 256;  // per CTA, or THREADS where a row takes more
 
-template <int THREADS>
-__device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t* red) {
+// Largest of the row's lanes; `turn` alternates so that a fast warp does not overwrite what a slow one still reads.
+template <int THREADS, int WARPS>
+__device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t (&red)[2][WARPS], int turn) {
   m = __reduce_max_sync(0xffffffffu, m);
   if constexpr (THREADS > 32) {
     constexpr int kWarps = THREADS / 32;
     const int warp = threadIdx.x / 32, first = warp / kWarps * kWarps;
-    if (threadIdx.x % 32 == 0) red[warp] = m;
+    if (threadIdx.x % 32 == 0) red[turn][warp] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) m = max(m, red[first + i]);
+    for (int i = 0; i < kWarps; ++i) m = max(m, red[turn][first + i]);
   }
   return m;
 }
 
-// KEEP: the row fits THREADS * NV chunks and stays in registers; otherwise it is read twice (the second time from L2
-// where it fits there).
-template <typename T, int THREADS, int NV, bool KEEP>
-__global__ void __launch_bounds__(THREADS > kQuantThreads ? THREADS : kQuantThreads) eb_quantize_kernel(QuantArgs a) {
-  constexpr int kBlock = THREADS > kQuantThreads ? THREADS : kQuantThreads;
-  constexpr int kRows = kBlock / THREADS;
-  __shared__ uint32_t red[kBlock / 32];
+template <int THREADS>
+constexpr int kQuantBlock = THREADS > kQuantThreads ? THREADS : kQuantThreads;
+
+template <typename T>
+__device__ __forceinline__ uint2 row_codes(const Raw<T>& raw, const RowScale& r) {
+  if (r.zero) return make_uint2(0, 0);
+  float v[8];
+  unpack(raw, v);
+  return codes8(v, r);
+}
+
+// Rows on 16-byte boundaries, THREADS * NV chunks long at most.  The grid walks the rows, and the next row is on its way
+// into a second set of registers while this one is rounded, so that memory is not idle between two rows.  Issue slots
+// come next: 8 instructions a value, where memory leaves room for about 11 at 16 bits.
+template <typename T, int THREADS, int NV>
+__global__ void __launch_bounds__(kQuantBlock<THREADS>, 1024 / kQuantBlock<THREADS>) eb_quantize_kernel(QuantArgs a) {
+  constexpr int kRows = kQuantBlock<THREADS> / THREADS;
+  __shared__ uint32_t red[2][kQuantBlock<THREADS> / 32];
   const int lane = threadIdx.x % THREADS;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
-  const bool live = row < a.rows;
-  const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_ld;
-  const int64_t cols = live ? a.cols : 0;
-  const int64_t chunks = (cols + 7) / 8;
-  Raw<T> keep[NV];
-  uint32_t m = 0;
-  for (int64_t base = 0; base < (KEEP ? 1 : chunks); base += THREADS * NV) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) keep[i] = load_chunk8(x, base + i * THREADS + lane, cols, a.wide_in);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) m = max(m, top_bits(keep[i]));
-  }
-  m = row_max<THREADS>(m, red);
-  if (!live) return;
-  const bool finite = m < 0x7f800000u;
-  const float top = __uint_as_float(m);
-  const float scale = finite ? __fdiv_rn(top, 127.0f) : top;
-  if (lane == 0) a.scale[row] = scale;
-  int8_t* q = a.q + row * a.q_ld;
-  // below 2^-100 the products above would lose bits: divided in 64 bits (half = 0 sends every chunk there)
-  const bool small = scale < 0x1p-100f;
-  const float inv = small ? 0.0f : __fdiv_rn(1.0f, scale), half = small ? 0.0f : 0.5f * scale;
-  const bool zero = !finite || scale == 0.0f;
-  for (int64_t base = 0; base < (KEEP ? 1 : chunks); base += THREADS * NV) {
+  const int whole = (int)(a.cols / 8), tail = (int)(a.cols % 8);
+  Raw<T> held[NV], next[NV];
+  auto fetch = [&](Raw<T>(&to)[NV], int64_t row) {
+    const T* at = static_cast<const T*>(a.x) + row * a.x_ld + lane * 8;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = base + i * THREADS + lane;
-      if (c >= chunks) break;
-      if constexpr (!KEEP) keep[i] = load_chunk8(x, c, cols, a.wide_in);
-      float v[8];
-      unpack(keep[i], v);
-      store_codes(a, q, c, zero ? make_uint2(0, 0) : codes8(v, scale, inv, half));
+      const int c = i * THREADS + lane;
+      if (c < whole)
+        to[i] = load_wide(at + i * THREADS * 8);
+      else
+        to[i] = load_values(at + i * THREADS * 8, c == whole ? tail : 0);
+    }
+  };
+  int turn = 0;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
+  const int64_t stride = (int64_t)gridDim.x * kRows;
+  if (row < a.rows) fetch(held, row);
+  // every thread of the CTA makes the same number of turns: they meet in row_max
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += stride, row += stride, turn ^= 1) {
+    const bool live = row < a.rows;
+    if (row + stride < a.rows) fetch(next, row + stride);
+    Top<T> top;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) widen(top, held[i]);
+    const uint32_t m = row_max<THREADS>(top_bits(top), red, turn);
+    if (live) {
+      const RowScale r = row_scale(m);
+      if (lane == 0) a.scale[row] = r.scale;
+      int8_t* to = a.q + row * a.q_ld + lane * 8;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * THREADS + lane;
+        if (c < whole)
+          __stcs(reinterpret_cast<uint2*>(to + i * THREADS * 8), row_codes(held[i], r));
+        else if (c == whole && tail)
+          store_codes(to + i * THREADS * 8, tail, row_codes(held[i], r));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) held[i] = next[i];
+  }
+}
+
+// Rows of any length and alignment, read twice (the second time from L2 where they fit there).
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) eb_quantize_any_kernel(QuantArgs a, bool wide) {
+  __shared__ uint32_t red[2][kQuantThreads / 32];
+  const int64_t chunks = (a.cols + 7) / 8;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+    auto load = [&](int64_t c) {
+      const int64_t left = a.cols - c * 8;
+      return wide && left >= 8 ? load_wide(x + c * 8) : load_values(x + c * 8, left < 8 ? (int)left : 8);
+    };
+    Top<T> top;
+    for (int64_t c = threadIdx.x; c < chunks; c += kQuantThreads) widen(top, load(c));
+    const RowScale r = row_scale(row_max<kQuantThreads>(top_bits(top), red, turn));
+    if (threadIdx.x == 0) a.scale[row] = r.scale;
+    int8_t* q = a.q + row * a.q_ld;
+    for (int64_t c = threadIdx.x; c < chunks; c += kQuantThreads) {
+      const int64_t left = a.cols - c * 8;
+      store_codes(q + c * 8, left < 8 ? (int)left : 8, row_codes(load(c), r));
     }
   }
 }
 
-template <typename T, int THREADS, int NV, bool KEEP = true>
-cudaError_t launch_quantize_as(const QuantArgs& a, cudaStream_t st) {
-  constexpr int kBlock = THREADS > kQuantThreads ? THREADS : kQuantThreads;
+template <typename T, int THREADS, int NV>
+cudaError_t launch_quantize_as(const QuantArgs& a, int sms, cudaStream_t st) {
+  constexpr int kBlock = kQuantBlock<THREADS>;
   constexpr int kRows = kBlock / THREADS;
-  eb_quantize_kernel<T, THREADS, NV, KEEP><<<(unsigned)((a.rows + kRows - 1) / kRows), kBlock, 0, st>>>(a);
+  int64_t grid = (a.rows + kRows - 1) / kRows;
+  const int64_t most = (int64_t)sms * (1024 / kBlock);
+  if (grid > most) grid = most;
+  eb_quantize_kernel<T, THREADS, NV><<<(unsigned)grid, kBlock, 0, st>>>(a);
   return cudaGetLastError();
 }
 
-// Lanes a row and chunks a lane: the fewest lanes that hold the row in 4 chunks each (8 for the longest rows).
+// The fewest lanes that hold the row in 64 bytes each: two sets of those and the arithmetic fit the 64 registers that
+// 1024 threads an SM leave each.
 template <typename T>
-cudaError_t launch_quantize(const QuantArgs& a, cudaStream_t st) {
+cudaError_t launch_quantize(const QuantArgs& a, bool wide_in, bool wide_out, int sms, cudaStream_t st) {
   const int64_t chunks = (a.cols + 7) / 8;
-  if (chunks <= 32) return launch_quantize_as<T, 32, 1>(a, st);
-  if (chunks <= 32 * 4) return launch_quantize_as<T, 32, 4>(a, st);
-  if (chunks <= 128 * 4) return launch_quantize_as<T, 128, 4>(a, st);
-  if (chunks <= 512 * 4) return launch_quantize_as<T, 512, 4>(a, st);
-  if (chunks <= 512 * 8) return launch_quantize_as<T, 512, 8>(a, st);
-  return launch_quantize_as<T, 512, 8, false>(a, st);
+  constexpr int kMost = sizeof(T) == 4 ? 2 : 4;
+  if (!wide_in || !wide_out || chunks > 1024 * kMost) {
+    const int64_t most = (int64_t)sms * 8;
+    eb_quantize_any_kernel<T><<<(unsigned)(a.rows < most ? a.rows : most), kQuantThreads, 0, st>>>(a, wide_in);
+    return cudaGetLastError();
+  }
+  if (chunks <= 32) return launch_quantize_as<T, 32, 1>(a, sms, st);
+  if (chunks <= 32 * kMost) return launch_quantize_as<T, 32, kMost>(a, sms, st);
+  if (chunks <= 128 * kMost) return launch_quantize_as<T, 128, kMost>(a, sms, st);
+  if (chunks <= 512 * kMost) return launch_quantize_as<T, 512, kMost>(a, sms, st);
+  return launch_quantize_as<T, 1024, kMost>(a, sms, st);
 }
 
 // ---- rows by expert ----------------------------------------------------------
@@ -449,12 +548,14 @@ int eb_quantize_rows(const void* x, int64_t rows, int64_t cols, int64_t x_ld, in
   a.cols = cols;
   a.x_ld = x_ld;
   a.q_ld = q_ld;
-  a.wide_in = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_ld * size % 16 == 0);
-  a.wide_out = reinterpret_cast<uintptr_t>(q) % 8 == 0 && (rows == 1 || q_ld % 8 == 0);
+  const bool wide_in = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_ld * size % 16 == 0);
+  const bool wide_out = reinterpret_cast<uintptr_t>(q) % 8 == 0 && (rows == 1 || q_ld % 8 == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = x_dtype == EB_OUT_F32    ? launch_quantize<float>(a, st)
-                        : x_dtype == EB_OUT_BF16 ? launch_quantize<__nv_bfloat16>(a, st)
-                                                 : launch_quantize<__half>(a, st);
+  const int sms = sm_count(device);
+  if (sms < 1) return linear_fail(EB_ERR_CUDA, "cannot read the SM count of device %d", device);
+  const cudaError_t e = x_dtype == EB_OUT_F32    ? launch_quantize<float>(a, wide_in, wide_out, sms, st)
+                        : x_dtype == EB_OUT_BF16 ? launch_quantize<__nv_bfloat16>(a, wide_in, wide_out, sms, st)
+                                                 : launch_quantize<__half>(a, wide_in, wide_out, sms, st);
   if (e != cudaSuccess) return linear_fail(EB_ERR_CUDA, "eb_quantize_rows: %s", cudaGetErrorString(e));
   return EB_OK;
 }

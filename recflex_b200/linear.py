@@ -74,43 +74,42 @@ def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _has_wide_rows(t: torch.Tensor) -> bool:
-    """Rows on 16-byte boundaries that do not overlap, as the products read them."""
-    size, k = t.element_size(), t.shape[-1]
-    if t.data_ptr() % 16 or (t.stride(-1) != 1 and k > 1):
-        return False
-    least = k
-    for d in range(t.dim() - 2, -1, -1):
-        if t.shape[d] > 1 and (t.stride(d) * size % 16 or t.stride(d) < least):
-            return False
-        if t.shape[d] > 1:
-            least = t.stride(d) * (t.shape[d] - 1) + least
-    return True
+def _wide_strides(t: torch.Tensor) -> Optional[Tuple[int, int]]:
+    """(elements between rows, elements between matrices) of `t` [..., rows, k] as the products read it: rows on 16-byte
+    boundaries that do not overlap.  None for any other layout.  Where there is one row or matrix, its stride is free
+    and reported as a packed tensor has it."""
+    shape, stride = t.shape, t.stride()
+    k, rows = shape[-1], shape[-2]
+    per = 16 // t.element_size()
+    if t.data_ptr() % 16 or (stride[-1] != 1 and k > 1):
+        return None
+    ld = stride[-2]
+    if rows <= 1:
+        ld = (k + per - 1) // per * per
+    elif ld < k or ld % per:
+        return None
+    group_ld = ld * max(1, rows)
+    if t.dim() == 3 and shape[0] > 1:
+        group_ld = stride[0]
+        if group_ld < ld * (rows - 1) + k or group_ld % per:
+            return None
+    return ld, group_ld
 
 
 def _empty_wide(shape, dtype: torch.dtype, device) -> torch.Tensor:
-    """Uninitialised [..., k] whose rows start on 16-byte boundaries."""
+    """Uninitialised [..., rows, k] whose rows start on 16-byte boundaries."""
     per = 16 // dtype.itemsize
-    k = shape[-1]
-    return torch.empty(tuple(shape[:-1]) + ((k + per - 1) // per * per,), dtype=dtype, device=device)[..., :k]
+    ld = (shape[-1] + per - 1) // per * per
+    strides = (ld, 1) if len(shape) == 2 else (ld * shape[1], ld, 1)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def pack_rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` [..., k] as it is if its rows start on 16-byte boundaries, otherwise a copy whose rows do.  The products
-    take any layout and make this copy themselves; weights are better laid out once."""
-    if _has_wide_rows(t):
+    """`t` [rows, k] or [experts, n, k] as it is if its rows start on 16-byte boundaries, otherwise a copy whose rows do.
+    The products take any layout and make this copy themselves; weights are better laid out once."""
+    if _wide_strides(t) is not None:
         return t
-    return _empty_wide(t.shape, t.dtype, t.device).copy_(t)
-
-
-def _row_stride(t: torch.Tensor, dim: int) -> int:
-    """Elements between neighbours of `dim`; where there is one entry only, what a packed tensor has."""
-    if t.shape[dim] > 1:
-        return t.stride(dim)
-    per = 16 // t.element_size()
-    if dim == t.dim() - 2:
-        return (t.shape[-1] + per - 1) // per * per
-    return _row_stride(t, dim + 1) * max(1, t.shape[dim + 1])
+    return _empty_wide(tuple(t.shape), t.dtype, t.device).copy_(t)
 
 
 def _span(t: torch.Tensor) -> Tuple[int, int]:
@@ -119,7 +118,8 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle, without the stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -134,7 +134,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if k > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < k:
         x = x.contiguous()
     q = _empty_wide((rows, k), torch.int8, x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    scale = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
     _lib.check(_lib.load().eb_quantize_rows(x.data_ptr(), rows, k, x.stride(0) if rows > 1 else k, _FLOATS[x.dtype],
                                             q.data_ptr(), q.stride(0) if rows > 1 else k, scale.data_ptr(),
                                             x.device.index, _stream(x.device)))
@@ -154,8 +154,8 @@ def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, tor
     rows, device, lib = groups.numel(), groups.device, _lib.load()
     need = C.c_size_t()
     _lib.check(lib.eb_group_rows_workspace_bytes(rows, int(num_groups), C.byref(need)))
-    order = torch.empty(rows, dtype=torch.int32, device=device)
-    offsets = torch.empty(int(num_groups) + 1, dtype=torch.int32, device=device)
+    order = torch.empty_strided((rows,), (1,), dtype=torch.int32, device=device)
+    offsets = torch.empty_strided((int(num_groups) + 1,), (1,), dtype=torch.int32, device=device)
     ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
     _lib.check(lib.eb_group_rows(groups.data_ptr(), rows, int(num_groups), _INDEX[groups.dtype], order.data_ptr(),
                                  offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, device.index,
@@ -212,9 +212,11 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     if out is None:
         # without out_rows every position is a row of the result, and the kernel fills those of no group with zeros
-        make = torch.empty if out_rows is None else torch.zeros
-        out = make((positions, n), dtype=out_dtype, device=device)
-        a.zero_rest = int(out_rows is None)
+        if out_rows is None:
+            out = torch.empty_strided((positions, n), (n, 1), dtype=out_dtype, device=device)
+            a.zero_rest = offsets is not None
+        else:
+            out = torch.zeros((positions, n), dtype=out_dtype, device=device)
     else:
         _check("out", out, 2, (out_dtype,), device)
         if out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
@@ -226,10 +228,16 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
             first, last = _span(t)
             if first < hi and lo < last:
                 raise ValueError("out must not share memory with the arguments")
-    x, weight = pack_rows(x), pack_rows(weight)
+    x_strides, w_strides = _wide_strides(x), _wide_strides(weight)
+    if x_strides is None:
+        x = pack_rows(x)
+        x_strides = _wide_strides(x)
+    if w_strides is None:
+        weight = pack_rows(weight)
+        w_strides = _wide_strides(weight)
     a.x, a.weight, a.out, a.status = x.data_ptr(), weight.data_ptr(), out.data_ptr(), _status_word(device).data_ptr()
-    a.x_rows, a.x_ld = x.shape[0], _row_stride(x, 0)
-    a.w_ld, a.w_group_ld = _row_stride(weight, weight.dim() - 2), _row_stride(weight, 0)
+    a.x_rows, a.x_ld = x.shape[0], x_strides[0]
+    a.w_ld, a.w_group_ld = w_strides
     a.positions, a.out_rows_total = positions, out.shape[0]
     a.out_ld = out.stride(0) if out.shape[0] > 1 else n
     a.n, a.k, a.num_groups = n, k, groups

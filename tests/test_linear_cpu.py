@@ -107,17 +107,17 @@ def test_host_tensors_are_refused():
 
 def test_wide_rows_are_recognised():
     """`pack_rows` copies exactly the layouts that the products cannot read in place, and keeps their values."""
+    wide = linear._wide_strides
     base = torch.arange(6 * 40, dtype=torch.int16).view(6, 40)
-    assert linear.pack_rows(base[:, :37]) is not None and linear._has_wide_rows(base[:, :37])
+    assert linear.pack_rows(base[:, :37]).data_ptr() == base.data_ptr() and wide(base[:, :37]) == (40, 240)
     for t in (base[:, 1:33], base.flatten()[: 5 * 41].view(5, 41), base[:, ::2], base.t(), base[:1].expand(6, 40)):
-        assert not linear._has_wide_rows(t)
+        assert wide(t) is None
         packed = linear.pack_rows(t)
-        assert linear._has_wide_rows(packed) and torch.equal(packed, t)
-    one = torch.zeros(1, 13, dtype=torch.int8)
-    assert linear._has_wide_rows(one) and linear._row_stride(one, 0) == 16
+        assert wide(packed) is not None and torch.equal(packed, t)
+    assert wide(torch.zeros(1, 13, dtype=torch.int8)) == (16, 16)
     cube = linear.pack_rows(torch.arange(3 * 5 * 7).view(3, 5, 7).to(torch.int8))
-    assert linear._has_wide_rows(cube) and linear._row_stride(cube, 1) == 16 and linear._row_stride(cube, 0) == 80
-    assert linear._row_stride(cube[:1], 0) == 80 and linear._row_stride(cube[:, :1], 1) == 16
+    assert wide(cube) == (16, 80) and wide(cube[:1]) == (16, 80) and wide(cube[:, :1]) == (16, 80)
+    assert wide(cube.transpose(0, 1)) is None and wide(cube[1:, 1:]) == (16, 80)
 
 
 def test_args_struct_matches_the_header(tmp_path):
