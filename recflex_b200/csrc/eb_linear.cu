@@ -27,13 +27,12 @@ namespace {
 using namespace mma;
 
 constexpr int kEpilogueWarps = 8;
-constexpr int kCopyWarps = 7;
-constexpr int kBoxWarps = 4;                           // that copy rows in order; rows by index take all of them
-constexpr int kFirstEpilogue = 32 * (kCopyWarps + 1);  // then one warp multiplies and the others store
+constexpr int kCopyWarps = 2;                          // and one that multiplies: 11 warps leave 168 registers a thread
+constexpr int kFirstEpilogue = 32 * (kCopyWarps + 1);
 constexpr int kThreads = kFirstEpilogue + 32 * kEpilogueWarps;
 constexpr int kKBytes = 128;                        // K of one stage: a row of the 128-byte swizzle
 constexpr int kABytes = 128 * kKBytes;
-constexpr int kBoxRows = 32;                        // rows of x per tensor copy: a ragged tile copies only its own boxes
+constexpr int kBoxRows = 128 / kCopyWarps;          // rows of x per tensor copy: a ragged tile copies only its own boxes
 constexpr int kColumnBytes = 1024;                  // per storing warp: scale and bias of its 128 columns
 constexpr int kSmemMax = 232448;
 constexpr int kMaxSplit = 8;                        // pieces of K: CTAs of the largest portable cluster
@@ -216,7 +215,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     eb_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_w) {
   using S = Shape<BN, CG>;
-  static_assert(kBoxRows * kBoxWarps == 128 && (CG == 1 || CG == 2), "rows of a CTA");
   static_assert(!SPLIT || CG == 1, "a pair of CTAs shares its tile already");
   constexpr int kStages = S::kStages;
   constexpr int kStep = I8 ? kKBytes : kKBytes / 2;  // elements of K per stage
@@ -236,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* tiles = off + a.num_groups + 1;
   static_assert(16 * kStages + 48 <= 256, "barriers");
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = CG > 1 || SPLIT ? cluster_rank() : 0;
   const bool leader = CG == 1 || rank == 0;
 
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kCopyWarps) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        bar_init(full + 8 * i, 1);
+        bar_init(full + 8 * i, CG * kCopyWarps);
         bar_init(empty + 8 * i, 1);
       }
       for (int i = 0; i < 2; ++i) {
@@ -285,69 +283,69 @@ __global__ void __launch_bounds__(kThreads, 1)
     return r;
   };
   auto rows_of = [&](const Tile& t, uint32_t r) { return min(max(t.m1 - t.m0 - (CG > 1 ? 128 * (int)r : 0), 0), 128); };
-  // bytes of x that CTA r copies per stage
-  auto bytes_of = [&](const Tile& t, uint32_t r) {
-    const int rows = rows_of(t, r);
-    return a.in_rows ? (rows + 3) / 4 * 4 * kKBytes : (rows + kBoxRows - 1) / kBoxRows * kBoxRows * kKBytes;
-  };
-
-  uint32_t copied = 0;  // stages filled so far (copying warps)
+  uint32_t copied = 0;  // stages filled so far (by the copying threads)
   if (warp < kCopyWarps) {
+    // One thread a warp; each takes its share of the rows of x, in order as one box, by index four at a time.  Each
+    // announces its own bytes for every stage, none where its rows do not exist: a stage is full only when all have
+    // passed its `empty` phase, so that none can fall a whole ring behind and take a later phase for its own.
+    constexpr int kQuads = 128 / 4 / kCopyWarps;
     bool ok = true;
-    const bool idle = !a.in_rows && warp >= kBoxWarps;
+    uint32_t st = 0, phase = 1;
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride) {
-      const Tile tile = tile_at(t);
-      const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
-      const int rows = rows_of(tile, rank);
-      uint32_t bytes = bytes_of(tile, 0) + CG * S::kParts * S::kWRows * kKBytes;
-      if constexpr (CG > 1) bytes += bytes_of(tile, 1);
-      // the copying warps share the rows: by index four at a time (a lane each), in order one box of 32 each.  (A warp's
-      // lanes issue their copies one after the other: by index, 4 warps took 639 us for 16384 x 15608 x 1024 in bf16 where
-      // 8 took 542 us, both on 256 x 256 tiles.  7 leave the other warps 128 registers.)
-      const int quad = lane * kCopyWarps + warp;
-      const bool copies = a.in_rows ? 4 * quad < rows : lane == 0 && kBoxRows * warp < rows;
-      int4 src = make_int4(0, 0, 0, 0);  // rows that do not exist read row 0: their products are not used
-      if (a.in_rows && copies) {
-        int* s = reinterpret_cast<int*>(&src);
+      if (elect_one()) {
+        const Tile tile = tile_at(t);
+        const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
+        const int first = warp * kBoxRows, mine = min(max(rows_of(tile, rank) - first, 0), kBoxRows);
+        const bool gather = a.in_rows != nullptr;
+        const uint32_t bytes = (gather ? (mine + 3) / 4 * 4 : mine > 0 ? kBoxRows : 0) * kKBytes + (warp < S::kParts ? S::kWRows * kKBytes : 0);
+        const int w_row = tile.n0 + warp * S::kPart + (CG > 1 ? S::kWRows * (int)rank : 0);
+        int4 src[kQuads];
+        if (gather) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * quad + j;
-          if (i < rows) {
-            const int r = __ldg(a.in_rows + m_cta + i);
-            s[j] = r >= 0 && r < a.x_rows ? r : 0;
+          for (int i = 0; i < 4 * kQuads; ++i) {  // rows that do not exist read row 0: their products are not used
+            int r = i < mine ? __ldg(a.in_rows + m_cta + first + i) : 0;
+            reinterpret_cast<int*>(src)[i] = r >= 0 && r < a.x_rows ? r : 0;
+          }
+        }
+        for (int k = k_first; k < k_last; ++k) {
+          ok = ok && bar_wait(empty + 8 * st, phase, gave_up);
+          if (!ok) break;
+          const uint32_t sx = ring + st * S::kStageBytes;
+          uint32_t bar = full + 8 * st;
+          if constexpr (CG > 1) {
+            bar = map_rank(bar, 0);
+            bar_expect_cluster(bar, bytes);
+          } else {
+            bar_expect(bar, bytes);
+          }
+          if (warp < S::kParts) load_3d<CG>(sx + kABytes + warp * S::kWRows * kKBytes, &map_w, k * kStep, w_row, tile.group, bar);
+          if (gather) {
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i)
+              if (4 * i < mine) load_rows4<CG>(sx + (first + 4 * i) * kKBytes, &map_x, k * kStep, src[i], bar);
+          } else if (mine > 0) {
+            load_2d<CG>(sx + first * kKBytes, &map_x, k * kStep, m_cta + first, bar);
+          }
+          ++copied;
+          if (++st == kStages) {
+            st = 0;
+            phase ^= 1;
           }
         }
       }
-      for (int k = k_first; k < k_last && ok && !idle; ++k) {
-        const uint32_t st = copied % kStages, phase = (copied / kStages) & 1;
-        ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * st, phase ^ 1, gave_up));
-        if (!ok) break;
-        const uint32_t sx = ring + st * S::kStageBytes, sw = sx + kABytes;
-        uint32_t bar = full + 8 * st;
-        if (leader && threadIdx.x == 0) bar_expect(bar, bytes);
-        if constexpr (CG > 1) bar = map_rank(bar, 0);
-        if (warp < S::kParts && lane == 0)
-          load_3d<CG>(sw + warp * S::kWRows * kKBytes, &map_w, k * kStep, tile.n0 + warp * S::kPart + (CG > 1 ? S::kWRows * (int)rank : 0), tile.group, bar);
-        if (copies) {
-          if (a.in_rows)
-            load_rows4<CG>(sx + quad * 4 * kKBytes, &map_x, k * kStep, src, bar);
-          else
-            load_2d<CG>(sx + warp * kBoxRows * kKBytes, &map_x, k * kStep, m_cta + kBoxRows * warp, bar);
-        }
-        ++copied;
-      }
+      ok = __all_sync(0xffffffffu, ok);
       if constexpr (SPLIT) {
-        __syncwarp();
         cluster_sync();
         cluster_sync();
       }
     }
   } else if (warp == kCopyWarps) {
     bool ok = true;
-    uint32_t used = 0, count = 0;
+    uint32_t count = 0, st = 0, phase = 0;
     const uint32_t desc = product_of(I8, a.dtype == EB_OUT_BF16, S::kRows, S::kPart);
-    auto wait_full = [&](uint32_t at) {
-      const bool there = bar_wait(full + 8 * (at % kStages), (at / kStages) & 1, gave_up);
+    const uint64_t x0 = operand(ring), w0 = operand(ring + kABytes);
+    auto wait_full = [&](uint32_t at, uint32_t parity) {
+      const bool there = bar_wait(full + 8 * at, parity, gave_up);
       fence_after();
       return there;
     };
@@ -357,41 +355,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       return there;
     };
     auto products = [&](uint32_t at, uint32_t slot, int part, bool add) {
-      const uint32_t x = ring + (at % kStages) * S::kStageBytes;
-      const uint64_t ax = operand(x), bw = operand(x + kABytes + part * S::kWRows * kKBytes);
+      const uint64_t x = x0 + at * (S::kStageBytes >> 4), w = w0 + at * (S::kStageBytes >> 4) + part * (S::kWRows * kKBytes >> 4);
 #pragma unroll
-      for (int i = 0; i < kKBytes / 32; ++i) multiply<I8, CG>(tmem + slot * S::kPart, ax + 2 * i, bw + 2 * i, desc, add || i > 0);
+      for (int i = 0; i < kKBytes / 32; ++i) multiply<I8, CG>(tmem + slot * S::kPart, x + 2 * i, w + 2 * i, desc, add || i > 0);
     };
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride, ++count) {
-      if (leader && lane == 0) {
+      if (leader && elect_one()) {
         const int steps = k_last - k_first;
         if constexpr (S::kParts == 1) {
           const uint32_t slot = count & 1;
           ok = ok && wait_drained(slot, count >> 1);
-          for (int k = 0; k < steps && ok; ++k, ++used) {
-            ok = wait_full(used);
+          for (int k = 0; k < steps; ++k) {
+            ok = ok && wait_full(st, phase);
             if (!ok) break;
-            products(used, slot, 0, k > 0);
-            commit<CG>(empty + 8 * (used % kStages));
+            products(st, slot, 0, k > 0);
+            commit<CG>(empty + 8 * st);
+            if (++st == kStages) {
+              st = 0;
+              phase ^= 1;
+            }
           }
           if (ok) commit<CG>(done + 8 * slot);
         } else {
           // the first stages' products with the first 256 columns run while the second 256 of the tile before are stored
           const int early = steps < kStages ? steps : kStages;
           ok = ok && wait_drained(0, count);
-          for (int k = 0; k < early && ok; ++k) {
-            ok = wait_full(used + k);
-            if (ok) products(used + k, 0, 0, k > 0);
+          uint32_t at = st, parity = phase;
+          for (int k = 0; k < early; ++k) {
+            ok = ok && wait_full(at, parity);
+            if (!ok) break;
+            products(at, 0, 0, k > 0);
+            if (++at == kStages) {
+              at = 0;
+              parity ^= 1;
+            }
           }
           ok = ok && wait_drained(1, count);
-          for (int k = 0; k < steps && ok; ++k, ++used) {
+          for (int k = 0; k < steps && ok; ++k) {
             if (k >= early) {
-              ok = wait_full(used);
+              ok = wait_full(st, phase);
               if (!ok) break;
-              products(used, 0, 0, true);
+              products(st, 0, 0, true);
             }
-            products(used, 1, 1, k > 0);
-            commit<CG>(empty + 8 * (used % kStages));
+            products(st, 1, 1, k > 0);
+            commit<CG>(empty + 8 * st);
+            if (++st == kStages) {
+              st = 0;
+              phase ^= 1;
+            }
           }
           if (ok) {
             commit<CG>(done);
@@ -399,18 +410,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      ok = __all_sync(0xffffffffu, ok);
       if constexpr (SPLIT) {
-        __syncwarp();
         cluster_sync();
         cluster_sync();
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-    if (leader && lane == 0 && !ok) {  // products in flight still read the ring
+    if (leader && !ok && elect_one()) {  // products in flight still read the ring
       volatile int keep = 0;
       commit<CG>(last);
       bar_wait(last, 0, &keep);
     }
+    __syncwarp();
   } else {
     const int e = warp - kCopyWarps - 1, quad = warp % 4, half = e / 4;
     const uint32_t mine = staging + e * S::kStaging;
@@ -570,8 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   __syncwarp();
   __syncthreads();
-  if (*gave_up && warp == 0) {
-    if (lane == 0) {
+  if (*gave_up && warp < kCopyWarps) {
+    if (elect_one()) {
       atomicOr(a.status, kLinearGaveUp);
       if (leader) {  // copies that are still on their way into the ring
         volatile int keep = 0;

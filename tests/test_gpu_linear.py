@@ -309,6 +309,32 @@ def test_grouped_linear_infinities_stay_in_their_rows(kind):
     assert (out[:2] == 0).all() and (out[-4:] == 0).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("k, n, groups", [(2048, 40, 150), (2048, 300, 60), (640, 130, 300), (8192, 600, 40)])
+def test_grouped_linear_many_ragged_tiles(kind, k, n, groups):
+    """Tiles of one row beside full ones, over and over: the copying warps that have nothing to copy for a tile keep
+    step with the others (one that fell a ring of stages behind would wait for good)."""
+    g = gen(k + n)
+    rng = np.random.default_rng(n)
+    sizes = rng.choice([0, 1, 2, 31, 33, 64, 65, 97, 128, 129, 200, 260], groups)
+    P, offsets = int(sizes.sum()), offsets_of(sizes)
+    kw = {}
+    if kind == "i8":
+        x, w = codes((P, k), g), codes((groups, n, k), g)
+        kw = dict(x_scale=scales(P, g), weight_scale=scales(groups * n, g).view(groups, n))
+    else:
+        x = torch.randn(P, k, generator=g, device=DEV).half()
+        w = (torch.randn(groups, n, k, generator=g, device=DEV) / k ** 0.5).half()
+    order = torch.randperm(P, generator=g, device=DEV).to(torch.int32)
+    for rows in (None, order):
+        want = linear.grouped_linear(x, w, offsets, in_rows=rows, **kw)
+        exact, slack = plain_grouped(x, w, offsets, None, "none", rows, None, want, kw.get("x_scale"), kw.get("weight_scale"))
+        check(want, exact, slack)
+        for _ in range(30):
+            assert torch.equal(linear.grouped_linear(x, w, offsets, in_rows=rows, **kw), want)
+    linear.check_status(DEV)
+
+
 def test_grouped_linear_repeated_rows():
     """Two experts a sample: the same row number twice in in_rows."""
     g = gen(12)
