@@ -27,15 +27,18 @@ namespace {
 using namespace mma;
 
 constexpr int kEpilogueWarps = 8;
-constexpr int kCopyWarps = 2;                          // and one that multiplies: 11 warps leave 168 registers a thread
+// Copies are issued one after the other by a warp's one thread: rows in order take 4 warps (a box of 32 rows each), rows
+// by index all 7 (a four-row copy takes its thread about 70 clocks: 2 warps took 705 us for 16384 x 15608 x 1024 in bf16
+// on 256 x 256 tiles, 4 took 541).  With the one that multiplies and those that store, 16 warps of 128 registers.
+constexpr int kCopyWarps = 7, kBoxWarps = 4;
 constexpr int kFirstEpilogue = 32 * (kCopyWarps + 1);
 constexpr int kThreads = kFirstEpilogue + 32 * kEpilogueWarps;
 constexpr int kKBytes = 128;                        // K of one stage: a row of the 128-byte swizzle
 constexpr int kABytes = 128 * kKBytes;
-constexpr int kBoxRows = 128 / kCopyWarps;          // rows of x per tensor copy: a ragged tile copies only its own boxes
+constexpr int kBoxRows = 128 / kBoxWarps;           // rows of x per tensor copy: a ragged tile copies only its own boxes
 constexpr int kColumnBytes = 1024;                  // per storing warp: scale and bias of its 128 columns
 constexpr int kSmemMax = 232448;
-constexpr int kMaxSplit = 8;                        // pieces of K: CTAs of the largest portable cluster
+constexpr int kMaxSplit = 4;                        // pieces of K (clusters of 8 such CTAs do not fill the SMs)
 
 template <int BN, int CG>
 struct Shape {
@@ -144,17 +147,18 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
   }
 #pragma unroll 1
   for (int c = 0; c < SPAN && n + c < a.n; c += kUnit) {
-    uint32_t v[kUnit];
-#pragma unroll
-    for (int i = 0; i < kUnit; i += kLoad) tmem_load(tm + c + i, *reinterpret_cast<uint32_t(*)[kLoad]>(v + i));
-    tmem_wait_load();
+    uint32_t v[kLoad];
     __syncwarp();  // the unit before has been read
-    if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) v[i] = 0;
-    }
 #pragma unroll
     for (int i = 0; i < kUnit; i += 8) {
+      if (i % kLoad == 0) {
+        tmem_load(tm + c + i, v);
+        tmem_wait_load();
+        if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
+#pragma unroll
+          for (int j = 0; j < kLoad; ++j) v[j] = 0;
+        }
+      }
       float2 o[4], f[4], b[4];
       *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(biases + c + i);
       *reinterpret_cast<float4*>(b + 2) = *reinterpret_cast<const float4*>(biases + c + i + 4);
@@ -164,7 +168,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t x = v[i + 2 * j], y = v[i + 2 * j + 1];
+        const uint32_t x = v[i % kLoad + 2 * j], y = v[i % kLoad + 2 * j + 1];
         if constexpr (I8)
           o[j] = fma2(make_float2((float)(int)x, (float)(int)y), mul2(row_scale, f[j]), b[j]);
         else
@@ -237,6 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = CG > 1 || SPLIT ? cluster_rank() : 0;
   const bool leader = CG == 1 || rank == 0;
+  const bool gather = a.in_rows != nullptr;
+  const int copiers = gather ? kCopyWarps : kBoxWarps;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kCopyWarps) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        bar_init(full + 8 * i, CG * kCopyWarps);
+        bar_init(full + 8 * i, CG * copiers);
         bar_init(empty + 8 * i, 1);
       }
       for (int i = 0; i < 2; ++i) {
@@ -288,23 +294,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One thread a warp; each takes its share of the rows of x, in order as one box, by index four at a time.  Each
     // announces its own bytes for every stage, none where its rows do not exist: a stage is full only when all have
     // passed its `empty` phase, so that none can fall a whole ring behind and take a later phase for its own.
-    constexpr int kQuads = 128 / 4 / kCopyWarps;
+    constexpr int kQuads = (32 + kCopyWarps - 1) / kCopyWarps;
     bool ok = true;
     uint32_t st = 0, phase = 1;
     for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride) {
-      if (elect_one()) {
+      if (warp < copiers && elect_one()) {
         const Tile tile = tile_at(t);
-        const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
-        const int first = warp * kBoxRows, mine = min(max(rows_of(tile, rank) - first, 0), kBoxRows);
-        const bool gather = a.in_rows != nullptr;
-        const uint32_t bytes = (gather ? (mine + 3) / 4 * 4 : mine > 0 ? kBoxRows : 0) * kKBytes + (warp < S::kParts ? S::kWRows * kKBytes : 0);
+        const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0), rows = rows_of(tile, rank);
+        const int quads = max(0, ((rows + 3) / 4 - warp + kCopyWarps - 1) / kCopyWarps);  // of this warp
+        const bool box = kBoxRows * warp < rows;
+        const uint32_t bytes = (gather ? 4 * quads : box ? kBoxRows : 0) * kKBytes + (warp < S::kParts ? S::kWRows * kKBytes : 0);
         const int w_row = tile.n0 + warp * S::kPart + (CG > 1 ? S::kWRows * (int)rank : 0);
         int4 src[kQuads];
         if (gather) {
 #pragma unroll
-          for (int i = 0; i < 4 * kQuads; ++i) {  // rows that do not exist read row 0: their products are not used
-            int r = i < mine ? __ldg(a.in_rows + m_cta + first + i) : 0;
-            reinterpret_cast<int*>(src)[i] = r >= 0 && r < a.x_rows ? r : 0;
+          for (int i = 0; i < kQuads; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // rows that do not exist read row 0: their products are not used
+              const int row = 4 * (i * kCopyWarps + warp) + j;
+              const int r = row < rows ? __ldg(a.in_rows + m_cta + row) : 0;
+              reinterpret_cast<int*>(src + i)[j] = r >= 0 && r < a.x_rows ? r : 0;
+            }
           }
         }
         for (int k = k_first; k < k_last; ++k) {
@@ -322,9 +332,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (gather) {
 #pragma unroll
             for (int i = 0; i < kQuads; ++i)
-              if (4 * i < mine) load_rows4<CG>(sx + (first + 4 * i) * kKBytes, &map_x, k * kStep, src[i], bar);
-          } else if (mine > 0) {
-            load_2d<CG>(sx + first * kKBytes, &map_x, k * kStep, m_cta + first, bar);
+              if (i < quads) load_rows4<CG>(sx + 4 * (i * kCopyWarps + warp) * kKBytes, &map_x, k * kStep, src[i], bar);
+          } else if (box) {
+            load_2d<CG>(sx + warp * kBoxRows * kKBytes, &map_x, k * kStep, m_cta + warp * kBoxRows, bar);
           }
           ++copied;
           if (++st == kStages) {
@@ -546,20 +556,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t at = ring + row * (BN * 4) + ((piece ^ (row & 7)) << 4);
             const RowInfo r = row_info<I8>(a, m_cta + row, tile.m1);
             uint32_t sum[4] = {};
+            uint4 part[kMaxSplit];
 #pragma unroll
-            for (int s0 = 0; s0 < kMaxSplit; s0 += 4) {  // four reads at a time on their way
-              uint4 part[4];
+            for (int s = 0; s < kMaxSplit; ++s)
+              if (s < pieces) part[s] = cluster_read(map_rank(at, s));
 #pragma unroll
-              for (int s = 0; s < 4; ++s)
-                if (s0 + s < pieces) part[s] = cluster_read(map_rank(at, s0 + s));
+            for (int s = 0; s < kMaxSplit; ++s) {
+              if (s >= pieces) break;
+              const uint32_t p[4] = {part[s].x, part[s].y, part[s].z, part[s].w};
 #pragma unroll
-              for (int s = 0; s < 4; ++s) {
-                if (s0 + s >= pieces) break;
-                const uint32_t p[4] = {part[s].x, part[s].y, part[s].z, part[s].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  sum[j] = I8 ? sum[j] + p[j] : __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(p[j]));
-              }
+              for (int j = 0; j < 4; ++j)
+                sum[j] = I8 ? sum[j] + p[j] : __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(p[j]));
             }
             if (r.dst < 0) continue;
 #pragma unroll
