@@ -688,18 +688,54 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   const int sms = sm_count(device);
   if (sms < 2) return linear_fail(EB_ERR_CUDA, "cannot read the SM count of device %d", device);
   args.k_steps = (int)(((int64_t)a.k * (I8 ? 1 : 2) + kKBytes - 1) / kKBytes);
+  // A few rows: one row of 15608 x 1024 takes 6.2 us in int8 (tiles with K split over 4 CTAs: 11.5), four 9.5 (12.0),
+  // eight 15.3 (11.2); six rows over 16 experts of 1924 x 1024 in fp16 9.1 (12.0), 32 over 64 22.4 (27.8), 64 over 64
+  // 52 (28): at most four rows, or half as many as there are experts.
+  if (a.positions <= 4 || 2 * a.positions <= a.num_groups) return launch_few(a, sms, st);
+  // One unit over rows of up to 256 bytes: 65536 rows of 128 int8 take 5.0 us (16-column tiles: 9.1), of 512 15.4 (9.9).
+  if (a.n == 1 && (int64_t)a.k * (I8 ? 1 : 2) <= 256) return launch_narrow(a, sms, st);
   const int64_t m128 = row_tiles(a, 128), m256 = row_tiles(a, 256);
-  if (a.positions <= kFewRows) return launch_few(a, sms, st);
-  if (a.n <= kNarrow) return launch_narrow(a, sms, st);
   if (a.n <= 16) return launch<I8, 16, 1, false>(args, device, sms, m128, 1, st);
-  const int64_t t64 = m128 * ((a.n + 63) / 64);
+  // The tile with the least estimated time: full waves of tiles (every group ends half a tile into its last one, on
+  // average) at so many clocks per stage of K, plus the clocks that a tile costs beside its products, plus those of
+  // storing the last one.  Wide tiles read x and the weights less often from L2, which bounds them; narrow ones give all
+  // SMs work.  Rows by index cannot be copied faster than 760 clocks per 128 of them and stage.  Clocks fitted to 29
+  // measured products (256 to 65536 rows, 256 to 15608 columns, 128 to 1024 units, 1 to 64 groups, int8 and bf16): the
+  // estimate's choice is within 2 % of the fastest tile for each of them, where no one tile is within 70 % for all.
+  struct Choice {
+    int rows, cols, ctas, stage, tile, last;
+  };
+  static const Choice choices[] = {{256, 512, 2, 1250, 7300, 4200}, {256, 256, 2, 630, 3100, 4700}, {128, 256, 1, 860, 3100, 1750},
+                                   {128, 128, 1, 410, 3100, 1200}, {128, 64, 1, 270, 3100, 0}};
+  const int64_t groups = a.num_groups < a.positions ? a.num_groups : a.positions;
+  auto clocks = [&](const Choice& c, int split) {
+    const int64_t tiles2 = (a.num_groups == 1 ? 2 * ((a.positions + c.rows - 1) / c.rows) : 2 * a.positions / c.rows + groups) * ((a.n + c.cols - 1) / c.cols);
+    const int64_t slots2 = 2 * (sms / (c.ctas * split));
+    const int64_t stage = a.in_rows && c.stage < 760 ? 760 : c.stage;
+    const int64_t body = (args.k_steps + split - 1) / split * stage + c.tile;
+    return (tiles2 + slots2 - 1) / slots2 * (body > c.last ? body : c.last) + c.last;
+  };
+  int best = 0;
+  for (int i = 1; i < 5; ++i)
+    if (clocks(choices[i], 1) < clocks(choices[best], 1)) best = i;
+  int64_t least = clocks(choices[best], 1);
+  // K split over 2 or 4 CTAs, where they all run at once: joining the sums costs about 3700 clocks
   int split = 1;
-  while (split < kMaxSplit && t64 * split * 2 <= sms && split * 2 <= args.k_steps) split *= 2;
+  for (int s = 2; s <= kMaxSplit; s *= 2) {
+    if (m128 * ((a.n + 63) / 64) * s > sms || s > args.k_steps) break;
+    if (clocks(choices[4], s) + 3700 < least) {
+      least = clocks(choices[4], s) + 3700;
+      split = s;
+    }
+  }
   if (split > 1) return launch<I8, 64, 1, true>(args, device, sms, m128, split, st);
-  if (t64 <= sms || a.n <= 64) return launch<I8, 64, 1, false>(args, device, sms, m128, 1, st);
-  if (a.n <= 128) return launch<I8, 128, 2, false>(args, device, sms, m256, 1, st);
-  if (a.n > 256 && args.k_steps >= 64) return launch<I8, 512, 2, false>(args, device, sms, m256, 1, st);
-  return launch<I8, 256, 2, false>(args, device, sms, m256, 1, st);
+  switch (best) {
+    case 0: return launch<I8, 512, 2, false>(args, device, sms, m256, 1, st);
+    case 1: return launch<I8, 256, 2, false>(args, device, sms, m256, 1, st);
+    case 2: return launch<I8, 256, 1, false>(args, device, sms, m128, 1, st);
+    case 3: return launch<I8, 128, 1, false>(args, device, sms, m128, 1, st);
+    default: return launch<I8, 64, 1, false>(args, device, sms, m128, 1, st);
+  }
 }
 
 }  // namespace

@@ -28,9 +28,7 @@ struct DeviceScope {
 
 constexpr int kMaxDevices = 64;
 
-// Products of at most this many positions, and of at most this many units, run on the ordinary arithmetic units.
-constexpr int kFewRows = 8;
-constexpr int kNarrow = 4;
+// Products on the ordinary arithmetic units (eb_linear_few.cu): of a few positions, and with one unit.
 int launch_few(const eb_linear_args& a, int sms, cudaStream_t st);
 int launch_narrow(const eb_linear_args& a, int sms, cudaStream_t st);
 

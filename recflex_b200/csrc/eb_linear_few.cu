@@ -1,6 +1,6 @@
 // Matrix products that the tensor units have no use for: a few rows (every
-// weight is read once, by as many loads in flight as it takes) and layers of a
-// few units (every row of x is read once).
+// weight is read once, by as many loads in flight as it takes) and layers of
+// one unit over short rows (every row of x is read once).
 #include "eb_linear.cuh"
 
 namespace ebk {
@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(kFewThreads) eb_linear_few_kernel(const __grid
   }
 }
 
-// Layers of at most UNITS units: `lanes` lanes share a row of x (each 16 bytes of it at a time), every lane set keeps 4
-// rows in flight.  Bound by the bytes of x; the weights come from L1.
-template <Kind KIND, int UNITS>
+// A layer of one unit over short rows: `lanes` lanes share a row of x (each 16 bytes of it at a time), every set of lanes
+// keeps 4 rows in flight.  Bound by the bytes of x; the weights come from L1.
+template <Kind KIND>
 __global__ void __launch_bounds__(kFewThreads) eb_linear_narrow_kernel(const __grid_constant__ eb_linear_args a, int lanes) {
   constexpr int kSize = KIND == kI8 ? 1 : 2, kPer = 16 / kSize, kRows = 4;
   __shared__ int off[EB_MAX_GROUPS + 1], tiles[EB_MAX_GROUPS + 1];
@@ -155,59 +155,43 @@ __global__ void __launch_bounds__(kFewThreads) eb_linear_narrow_kernel(const __g
   if (a.zero_rest) zero_rest(a, off, (int64_t)blockIdx.x * kFewThreads + threadIdx.x, (int64_t)gridDim.x * kFewThreads);
   const int first = off[0], live = off[a.num_groups] - first;
   for (int64_t base = (int64_t)blockIdx.x * sets * kRows; base < live; base += (int64_t)gridDim.x * sets * kRows) {
-    const uint8_t *x[kRows], *w[kRows];
+    const uint8_t* x[kRows];
     int pos[kRows], group[kRows];
-    Sum<KIND> acc[kRows][UNITS] = {};
+    Sum<KIND> acc[kRows] = {};
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int64_t i = base + r * sets + set;
       pos[r] = i < live ? first + (int)i : -1;
       group[r] = i < live && a.num_groups > 1 ? find_group(tiles, a.num_groups, (int)i) : 0;
       x[r] = i < live ? row_of(a, pos[r], kSize) : nullptr;
-      w[r] = static_cast<const uint8_t*>(a.weight) + (int64_t)group[r] * a.w_group_ld * kSize;
+      if (!x[r]) x[r] = static_cast<const uint8_t*>(a.weight);  // a row of the right length whose products are not used
     }
-    for (int64_t e = lane * kPer; e < a.k; e += lanes * kPer) {
+    for (int e = lane * kPer; e < a.k; e += lanes * kPer) {
       uint4 xv[kRows];
 #pragma unroll
+      for (int r = 0; r < kRows; ++r) xv[r] = load_piece<KIND>(x[r], e, a.k);
+#pragma unroll
       for (int r = 0; r < kRows; ++r)
-        if (x[r]) xv[r] = load_piece<KIND>(x[r], (int)e, a.k);
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        if (!x[r]) continue;
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-          if (u < a.n) add_products<KIND>(acc[r][u], xv[r], load_piece<KIND>(w[r] + u * a.w_ld * kSize, (int)e, a.k));
-      }
+        add_products<KIND>(acc[r], xv[r], load_piece<KIND>(static_cast<const uint8_t*>(a.weight) + (int64_t)group[r] * a.w_group_ld * kSize, e, a.k));
     }
     __syncwarp();
+    Sum<KIND> v = 0;
+    int p = -1, g = 0;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) acc[r][u] = warp_sum<KIND>(acc[r][u], lanes);
-    if (lane < kRows) {  // one lane a row (a set has at least 4 lanes)
-      Sum<KIND> v[UNITS];
-      int p = -1, g = 0;
-#pragma unroll
-      for (int r = 0; r < kRows; ++r)
-        if (lane == r) {
-          p = pos[r];
-          g = group[r];
-#pragma unroll
-          for (int u = 0; u < UNITS; ++u) v[u] = acc[r][u];
-        }
-      if (p >= 0) {
-        const RowInfo info = row_info<KIND == kI8>(a, p, p + 1);
-        if (info.dst >= 0) {
-#pragma unroll
-          for (int u = 0; u < UNITS; ++u)
-            if (u < a.n) {
-              const int64_t c = (int64_t)g * a.n + u;
-              store_value(a.out, (int64_t)info.dst * a.out_ld + u, a.out_dtype,
-                          finish<KIND == kI8>(sum_bits<KIND>(v[u]), info, KIND == kI8 ? __ldg(a.w_scale + c) : 1.0f,
-                                              a.bias ? __ldg(a.bias + c) : 0.0f, a.activation));
-            }
-        }
+    for (int r = 0; r < kRows; ++r) {
+      const Sum<KIND> sum = warp_sum<KIND>(acc[r], lanes);
+      if (lane == r) {  // one lane a row (a set has at least 4 lanes)
+        v = sum;
+        p = pos[r];
+        g = group[r];
       }
+    }
+    if (p >= 0) {
+      const RowInfo info = row_info<KIND == kI8>(a, p, p + 1);
+      if (info.dst >= 0)
+        store_value(a.out, (int64_t)info.dst * a.out_ld, a.out_dtype,
+                    finish<KIND == kI8>(sum_bits<KIND>(v), info, KIND == kI8 ? __ldg(a.w_scale + g) : 1.0f,
+                                        a.bias ? __ldg(a.bias + g) : 0.0f, a.activation));
     }
     __syncwarp();
   }
@@ -219,7 +203,7 @@ cudaError_t few(const eb_linear_args& a, int sms, cudaStream_t st) {
   // tiles, whose weights are then read from L2)
   int64_t most = a.num_groups == 1 ? a.positions : 2 * a.positions / a.num_groups + 1;
   if (most > a.positions) most = a.positions;
-  const int rows = most <= 1 ? 1 : most <= 2 ? 2 : most <= 4 ? 4 : 8;
+  const int rows = most <= 1 ? 1 : most <= 2 ? 2 : 4;
   const int64_t tiles = row_tiles(a, rows);
   // warps that split K: until each has 4 KB of a row or less to read and every SM has a CTA
   const int pieces = (int)(((int64_t)a.k * (KIND == kI8 ? 1 : 2) + 511) / 512);
@@ -231,10 +215,8 @@ cudaError_t few(const eb_linear_args& a, int sms, cudaStream_t st) {
     eb_linear_few_kernel<KIND, 1><<<grid, kFewThreads, 0, st>>>(a, share);
   else if (rows == 2)
     eb_linear_few_kernel<KIND, 2><<<grid, kFewThreads, 0, st>>>(a, share);
-  else if (rows == 4)
-    eb_linear_few_kernel<KIND, 4><<<grid, kFewThreads, 0, st>>>(a, share);
   else
-    eb_linear_few_kernel<KIND, 8><<<grid, kFewThreads, 0, st>>>(a, share);
+    eb_linear_few_kernel<KIND, 4><<<grid, kFewThreads, 0, st>>>(a, share);
   return cudaGetLastError();
 }
 
@@ -245,10 +227,7 @@ cudaError_t narrow(const eb_linear_args& a, int sms, cudaStream_t st) {
   const int64_t rows = kFewThreads / lanes * 4;
   int64_t grid = (a.positions + rows - 1) / rows;
   if (grid > (int64_t)sms * 8) grid = (int64_t)sms * 8;
-  if (a.n == 1)
-    eb_linear_narrow_kernel<KIND, 1><<<(unsigned)grid, kFewThreads, 0, st>>>(a, lanes);
-  else
-    eb_linear_narrow_kernel<KIND, 4><<<(unsigned)grid, kFewThreads, 0, st>>>(a, lanes);
+  eb_linear_narrow_kernel<KIND><<<(unsigned)grid, kFewThreads, 0, st>>>(a, lanes);
   return cudaGetLastError();
 }
 

@@ -336,29 +336,59 @@ cudaError_t launch_quantize(const QuantArgs& a, bool wide_in, bool wide_out, int
 // A stable counting sort.  Every warp owns one contiguous run of rows and counts it by expert (the lanes that hold
 // the same expert add as one); an exclusive scan over (expert, warp), experts outermost, turns the counts into the
 // place of each warp's first row of each expert; and each warp walks its run again and places its rows in order.
-// There are no atomics between warps: the order is the same on every run.
+// The places follow from the counts alone: the order is the same on every run.  Up to 4096 rows one CTA does all of it;
+// above, a first kernel counts the rows of every CTA by expert, and the CTAs of the second add up what the others
+// counted, count their own rows again by warp and place them.  Latency is what costs; the scattered stores want all
+// SMs (one cluster of 8 CTAs took 28 us for 131072 rows of 64 experts).  The lanes of the same expert are found with a
+// vote per bit of the expert number; the match instruction, which gives them at once, took longer.
 
 constexpr int kGroupThreads = 1024;
-constexpr int kGroupWarps = kGroupThreads / 32;
-constexpr int64_t kOneCtaRows = 16384;  // up to here one CTA does all three steps
+constexpr int kAhead = 4;
 
 template <typename I>
-__device__ __forceinline__ int group_of(const I* __restrict__ groups, int64_t r, int num_groups) {
-  const long long g = (long long)groups[r];
+__device__ __forceinline__ int group_of(I g, int num_groups) {
   return g < 0 || g >= num_groups ? num_groups : (int)g;
+}
+
+// The lanes whose g equals this one's, among those with g >= 0; g < 2^bits.
+__device__ __forceinline__ unsigned same_group(int g, int bits) {
+  unsigned same = __ballot_sync(0xffffffffu, g >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned ones = __ballot_sync(0xffffffffu, (g >> b) & 1);
+    same &= (g >> b) & 1 ? ones : ~ones;
+  }
+  return same;
+}
+
+// Calls each(row, group, lanes of the same group) for rows [first, last) in order, 32 at a time; -1 behind the last.
+template <typename I, typename F>
+__device__ __forceinline__ void walk_rows(const I* __restrict__ groups, int64_t first, int64_t last, int num_groups, F each) {
+  const int lane = threadIdx.x % 32, bits = 32 - __clz(num_groups);
+  for (int64_t r0 = first; r0 < last; r0 += 32 * kAhead) {
+    I held[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + 32 * i + lane;
+      held[i] = r < last ? groups[r] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (r0 + 32 * i >= last) break;
+      const int64_t r = r0 + 32 * i + lane;
+      const int g = r < last ? group_of(held[i], num_groups) : -1;
+      each(r, g, same_group(g, bits));
+    }
+  }
 }
 
 // Counts rows [first, last) into cnt[0..num_groups] (this warp's own).
 template <typename I>
 __device__ __forceinline__ void warp_count(const I* groups, int64_t first, int64_t last, int num_groups, uint32_t* cnt) {
   const int lane = threadIdx.x % 32;
-  for (int64_t r0 = first; r0 < last; r0 += 32) {
-    const int64_t r = r0 + lane;
-    const int g = r < last ? group_of(groups, r, num_groups) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, g);
+  walk_rows(groups, first, last, num_groups, [&](int64_t, int g, unsigned same) {
     if (g >= 0 && lane == __ffs(same) - 1) cnt[g] += __popc(same);
     __syncwarp();
-  }
+  });
 }
 
 // Places rows [first, last): cnt holds the next place of each expert's rows of this warp.
@@ -366,10 +396,7 @@ template <typename I>
 __device__ __forceinline__ void warp_place(const I* groups, int64_t first, int64_t last, int num_groups, uint32_t* cnt,
                                            int32_t* order) {
   const int lane = threadIdx.x % 32;
-  for (int64_t r0 = first; r0 < last; r0 += 32) {
-    const int64_t r = r0 + lane;
-    const int g = r < last ? group_of(groups, r, num_groups) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, g);
+  walk_rows(groups, first, last, num_groups, [&](int64_t r, int g, unsigned same) {
     const uint32_t at = g >= 0 ? cnt[g] : 0;
     __syncwarp();
     if (g >= 0) {
@@ -377,16 +404,16 @@ __device__ __forceinline__ void warp_place(const I* groups, int64_t first, int64
       if (lane == __ffs(same) - 1) cnt[g] = at + __popc(same);
     }
     __syncwarp();
-  }
+  });
 }
 
-// Exclusive scan in place over n values at v (one CTA of kGroupThreads threads; `part` holds one value per warp).
-__device__ __forceinline__ void cta_scan(uint32_t* v, int64_t n, uint32_t* part) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t each = (n + kGroupThreads - 1) / kGroupThreads;
-  const int64_t first = min(n, (int64_t)threadIdx.x * each), last = min(n, first + each);
+// Exclusive scan in place over n values at v, by all threads of a CTA (`part` holds one value per warp).
+__device__ __forceinline__ void cta_scan(uint32_t* v, int n, uint32_t* part) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int each = (n + blockDim.x - 1) / blockDim.x;
+  const int first = min(n, (int)threadIdx.x * each), last = min(n, first + each);
   uint32_t sum = 0;
-  for (int64_t i = first; i < last; ++i) sum += v[i];
+  for (int i = first; i < last; ++i) sum += v[i];
   uint32_t run = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -395,19 +422,10 @@ __device__ __forceinline__ void cta_scan(uint32_t* v, int64_t n, uint32_t* part)
   }
   if (lane == 31) part[warp] = run;
   __syncthreads();
-  if (warp == 0) {
-    uint32_t p = lane < kGroupWarps ? part[lane] : 0;
-    const uint32_t own = p;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, p, d);
-      if (lane >= d) p += o;
-    }
-    part[lane] = p - own;
-  }
-  __syncthreads();
-  uint32_t at = part[warp] + run - sum;
-  for (int64_t i = first; i < last; ++i) {
+  uint32_t at = run - sum;
+  const uint32_t p = lane < warps && lane < warp ? part[lane] : 0;
+  at += __reduce_add_sync(0xffffffffu, p);
+  for (int i = first; i < last; ++i) {
     const uint32_t c = v[i];
     v[i] = at;
     at += c;
@@ -415,108 +433,124 @@ __device__ __forceinline__ void cta_scan(uint32_t* v, int64_t n, uint32_t* part)
   __syncthreads();
 }
 
+struct GroupArgs {
+  int64_t rows;
+  int64_t each;      // rows of a CTA
+  int num_groups, warps;  // warps of a CTA that take rows
+  uint32_t* table;   // [CTAs][experts + 1]: rows of each CTA
+  int32_t *order, *offsets;
+};
+
+// The CTA's rows counted by warp: cnt[warp][expert]
 template <typename I>
-__global__ void __launch_bounds__(kGroupThreads) eb_group_small_kernel(const I* __restrict__ groups, int rows,
-                                                                       int num_groups, int warps, int32_t* order,
-                                                                       int32_t* offsets) {
-  extern __shared__ uint32_t cnt[];
-  __shared__ uint32_t part[32];
-  const int warp = threadIdx.x / 32;
-  const int bins = num_groups + 1;
-  uint32_t* mine = cnt + (size_t)warp * bins;                 // counts, warp by warp
-  uint32_t* place = cnt + (size_t)warps * bins;               // the same, expert by expert
-  const int each = ((rows + warps - 1) / warps + 31) / 32 * 32;
-  const int64_t first = min((int64_t)rows, (int64_t)warp * each), last = min((int64_t)rows, first + each);
-  for (int i = threadIdx.x; i < warps * bins; i += kGroupThreads) cnt[i] = 0;
+__device__ __forceinline__ void cta_count(const I* groups, const GroupArgs& a, uint32_t* cnt, int64_t& first, int64_t& last) {
+  const int warp = threadIdx.x / 32, bins = a.num_groups + 1;
+  const int64_t begin = min(a.rows, (int64_t)blockIdx.x * a.each), end = min(a.rows, begin + a.each);
+  const int64_t run = ((a.each + a.warps - 1) / a.warps + 31) / 32 * 32;
+  first = min(end, begin + warp * run), last = warp < a.warps ? min(end, first + run) : first;
+  for (int i = threadIdx.x; i < a.warps * bins; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  if (warp < warps) warp_count(groups, first, last, num_groups, mine);
+  if (warp < a.warps) warp_count(groups, first, last, a.num_groups, cnt + warp * bins);
   __syncthreads();
-  for (int i = threadIdx.x; i < warps * bins; i += kGroupThreads) place[i] = cnt[(size_t)(i % warps) * bins + i / warps];
-  __syncthreads();
-  cta_scan(place, (int64_t)warps * bins, part);
-  for (int i = threadIdx.x; i < warps * bins; i += kGroupThreads) cnt[(size_t)(i % warps) * bins + i / warps] = place[i];
-  for (int g = threadIdx.x; g < bins; g += kGroupThreads)
-    if (g <= num_groups) offsets[g] = (int32_t)place[(size_t)g * warps];
-  __syncthreads();
-  if (warp < warps) warp_place(groups, first, last, num_groups, mine, order);
 }
 
-// Larger inputs: counts to the workspace as [num_groups + 1][warps], scanned by one CTA.
-constexpr int kPlaceThreads = 256;
-constexpr int kPlaceWarps = kPlaceThreads / 32;
-
-template <typename I, bool PLACE>
-__global__ void __launch_bounds__(kPlaceThreads) eb_group_rows_kernel(const I* __restrict__ groups, int64_t rows,
-                                                                      int64_t each, int num_groups, int64_t warps,
-                                                                      uint32_t* table, int32_t* order) {
-  extern __shared__ uint32_t cnt[];  // [kPlaceWarps][num_groups + 1]
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int bins = num_groups + 1;
-  uint32_t* mine = cnt + (size_t)warp * bins;
-  const int64_t w = (int64_t)blockIdx.x * kPlaceWarps + warp;
-  const int64_t first = min(rows, w * each), last = min(rows, first + each);
-  if (w >= warps) return;
-  for (int g = lane; g < bins; g += 32) mine[g] = PLACE ? table[(size_t)g * warps + w] : 0;
-  __syncwarp();
-  if constexpr (PLACE) {
-    warp_place(groups, first, last, num_groups, mine, order);
-  } else {
-    warp_count(groups, first, last, num_groups, mine);
-    for (int g = lane; g < bins; g += 32) table[(size_t)g * warps + w] = mine[g];
+template <typename I>
+__global__ void __launch_bounds__(kGroupThreads) eb_group_count_kernel(const I* __restrict__ groups, const GroupArgs a) {
+  extern __shared__ uint32_t cnt[];
+  const int bins = a.num_groups + 1;
+  int64_t first, last;
+  cta_count(groups, a, cnt, first, last);
+  for (int g = threadIdx.x; g < bins; g += blockDim.x) {
+    uint32_t sum = 0;
+    for (int w = 0; w < a.warps; ++w) sum += cnt[w * bins + g];
+    a.table[(size_t)blockIdx.x * bins + g] = sum;
   }
 }
 
-__global__ void __launch_bounds__(kGroupThreads) eb_group_scan_kernel(uint32_t* table, int64_t warps, int num_groups,
-                                                                      int32_t* offsets) {
+// Shared memory: counts [warps][experts + 1], rows of each expert in the CTAs before, rows of each expert in all.
+template <typename I>
+__global__ void __launch_bounds__(kGroupThreads) eb_group_place_kernel(const I* __restrict__ groups, const GroupArgs a) {
+  extern __shared__ uint32_t cnt[];
   __shared__ uint32_t part[32];
-  cta_scan(table, warps * (num_groups + 1), part);
-  for (int g = threadIdx.x; g <= num_groups; g += kGroupThreads) offsets[g] = (int32_t)table[(size_t)g * warps];
+  const int warp = threadIdx.x / 32, bins = a.num_groups + 1;
+  uint32_t* before = cnt + a.warps * bins;
+  uint32_t* base = before + bins;
+  for (int i = threadIdx.x; i < 2 * bins; i += blockDim.x) before[i] = 0;
+  int64_t first, last;
+  cta_count(groups, a, cnt, first, last);
+  if (gridDim.x > 1) {  // sums of whole numbers: the order of the additions does not matter
+    for (int i = threadIdx.x; i < bins * (int)gridDim.x; i += blockDim.x) {
+      const uint32_t v = a.table[i];
+      const int c = i / bins, g = i - c * bins;
+      atomicAdd(base + g, v);
+      if (c < (int)blockIdx.x) atomicAdd(before + g, v);
+    }
+    __syncthreads();
+  }
+  for (int g = threadIdx.x; g < bins; g += blockDim.x) {  // rows in the CTAs and warps before
+    uint32_t sum = before[g];
+    for (int w = 0; w < a.warps; ++w) {
+      const uint32_t c = cnt[w * bins + g];
+      cnt[w * bins + g] = sum;
+      sum += c;
+    }
+    if (gridDim.x == 1) base[g] = sum;
+  }
+  __syncthreads();
+  cta_scan(base, bins, part);
+  for (int i = threadIdx.x; i < a.warps * bins; i += blockDim.x) cnt[i] += base[i % bins];
+  if (blockIdx.x == 0)
+    for (int g = threadIdx.x; g < bins; g += blockDim.x) a.offsets[g] = (int32_t)base[g];
+  __syncthreads();
+  if (warp < a.warps) warp_place(groups, first, last, a.num_groups, cnt + warp * bins, a.order);
 }
 
+constexpr int64_t kOneCtaRows = 4096;
+constexpr int kGroupSmem = 200 * 1024;
+
 struct GroupPlan {
-  bool small;
-  int64_t warps, each;
-  size_t bytes;
+  int ctas, threads;
+  GroupArgs args;
+  size_t bytes;  // workspace
 };
 
 GroupPlan group_plan(int64_t rows, int num_groups) {
   GroupPlan p{};
   const int64_t bins = num_groups + 1;
-  // one CTA holds two tables of warps x experts in its shared memory
-  const int64_t fit = (200 * 1024) / (8 * bins);
-  p.small = rows <= kOneCtaRows;
-  if (p.small) {
-    p.warps = (rows + 127) / 128;
-    if (p.warps > kGroupWarps) p.warps = kGroupWarps;
-    if (p.warps > fit) p.warps = fit;
-    if (p.warps < 1) p.warps = 1;
-    return p;
+  p.ctas = 1;
+  p.threads = rows <= 1024 ? 256 : kGroupThreads;
+  if (rows > kOneCtaRows) {
+    // a CTA for every 1024 rows, as far as its look at all CTAs' counts stays short
+    int64_t most = 65536 / bins;
+    most = most > 128 ? 128 : most;
+    const int64_t want = (rows + 1023) / 1024;
+    p.ctas = (int)(want < most ? want : most);
+    p.bytes = (size_t)p.ctas * bins * sizeof(uint32_t);
   }
-  // runs of 512 rows, longer where the table of counts would outgrow what one CTA scans quickly
-  p.each = 512;
-  while ((rows + p.each - 1) / p.each * bins > 65536 && p.each < rows) p.each *= 2;
-  p.warps = (rows + p.each - 1) / p.each;
-  p.bytes = (size_t)(p.warps * bins) * sizeof(uint32_t);
+  p.args.rows = rows;
+  p.args.each = (rows + p.ctas - 1) / p.ctas;
+  p.args.num_groups = num_groups;
+  int64_t warps = p.threads / 32;
+  const int64_t fit = kGroupSmem / (4 * bins) - 2, need = (p.args.each + 31) / 32;
+  if (warps > fit) warps = fit;
+  if (warps > need) warps = need;
+  p.args.warps = (int)(warps < 1 ? 1 : warps);
   return p;
 }
 
 template <typename I>
-cudaError_t launch_group(const void* groups, int64_t rows, int num_groups, int32_t* order, int32_t* offsets,
-                         const GroupPlan& p, uint32_t* table, cudaStream_t st) {
+cudaError_t launch_group(const void* groups, GroupPlan& p, cudaStream_t st) {
+  static_assert(kGroupSmem / (4 * (EB_MAX_GROUPS + 1)) - 2 >= 1, "the tables of one warp fit");
   const I* g = static_cast<const I*>(groups);
-  const int bins = num_groups + 1;
-  if (p.small) {
-    const size_t smem = (size_t)p.warps * bins * 8;
-    cudaError_t e = cudaFuncSetAttribute(eb_group_small_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  const size_t bins = p.args.num_groups + 1;
+  const size_t smem = (p.args.warps + 2) * bins * 4;
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(eb_group_count_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(eb_group_place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmem);
     if (e != cudaSuccess) return e;
-    eb_group_small_kernel<I><<<1, kGroupThreads, smem, st>>>(g, (int)rows, num_groups, (int)p.warps, order, offsets);
-    return cudaGetLastError();
   }
-  const size_t smem = (size_t)kPlaceWarps * bins * 4;
-  const unsigned grid = (unsigned)((p.warps + kPlaceWarps - 1) / kPlaceWarps);
-  eb_group_rows_kernel<I, false><<<grid, kPlaceThreads, smem, st>>>(g, rows, p.each, num_groups, p.warps, table, order);
-  eb_group_scan_kernel<<<1, kGroupThreads, 0, st>>>(table, p.warps, num_groups, offsets);
-  eb_group_rows_kernel<I, true><<<grid, kPlaceThreads, smem, st>>>(g, rows, p.each, num_groups, p.warps, table, order);
+  if (p.ctas > 1) eb_group_count_kernel<I><<<p.ctas, p.threads, smem, st>>>(g, p.args);
+  eb_group_place_kernel<I><<<p.ctas, p.threads, smem, st>>>(g, p.args);
   return cudaGetLastError();
 }
 
@@ -580,11 +614,12 @@ int eb_group_rows(const void* groups, int64_t rows, int num_groups, int index_dt
     return linear_fail(EB_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   DeviceScope scope(device);
   if (!scope.ok) return linear_fail(EB_ERR_CUDA, "cannot select device %d", device);
-  const GroupPlan p = group_plan(rows, num_groups);
+  GroupPlan p = group_plan(rows, num_groups);
+  p.args.table = static_cast<uint32_t*>(workspace);
+  p.args.order = order;
+  p.args.offsets = offsets;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = index_dtype == EB_I64
-                            ? launch_group<long long>(groups, rows, num_groups, order, offsets, p, static_cast<uint32_t*>(workspace), st)
-                            : launch_group<int>(groups, rows, num_groups, order, offsets, p, static_cast<uint32_t*>(workspace), st);
+  const cudaError_t e = index_dtype == EB_I64 ? launch_group<long long>(groups, p, st) : launch_group<int>(groups, p, st);
   if (e != cudaSuccess) return linear_fail(EB_ERR_CUDA, "eb_group_rows: %s", cudaGetErrorString(e));
   return EB_OK;
 }
