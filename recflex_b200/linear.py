@@ -25,36 +25,39 @@ _ACTIVATIONS = {"none": _lib.EB_ACT_NONE, "relu": _lib.EB_ACT_RELU, "sigmoid": _
 _INDEX = {torch.int32: _lib.EB_I32, torch.int64: _lib.EB_I64}
 
 _status_lock = threading.Lock()
-_status = {}
+_status = {}  # device index: (its status word, the word's address)
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
-    """The device's status word, made at the first call.  Calls only set bits in it, so all streams share it."""
-    word = _status.get(device)
+def _status_word(index: int) -> int:
+    """Address of the device's status word, made at the first call.  Calls only set bits in it: all streams share it."""
+    word = _status.get(index)
     if word is None:
         with _status_lock:
-            word = _status.get(device)
+            word = _status.get(index)
             if word is None:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the first call on a device must come before any stream capture")
-                word = torch.zeros(1, dtype=torch.int32, device=device)
-                torch.cuda.current_stream(device).synchronize()
-                _status[device] = word
-    return word
+                t = torch.zeros(1, dtype=torch.int32, device=f"cuda:{index}")
+                torch.cuda.current_stream(index).synchronize()
+                word = _status[index] = (t, t.data_ptr())
+    return word[1]
 
 
 def check_status(device=None) -> None:
     """Raise if a product since the last check met offsets or row numbers outside their range (synchronises)."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if device.type == "cuda" and device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    word = _status.get(device)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"check_status needs a CUDA device, got {device}")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    word = _status.get(index)
     if word is not None:
-        _lib.check(_lib.load().eb_linear_check_status(word.data_ptr(), device.index,
-                                                      torch.cuda.current_stream(device).cuda_stream))
+        _lib.check(_lib.load().eb_linear_check_status(word[1], index, torch.cuda.current_stream(index).cuda_stream))
 
 
 def _check(name: str, t: torch.Tensor, dims: int, dtypes, device: Optional[torch.device] = None) -> None:
+    if type(t) is torch.Tensor and t.is_cuda and t.dim() == dims and t.dtype in dtypes and not t.requires_grad \
+            and (device is None or t.get_device() == device.index):
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if device is not None and t.device != device:
@@ -68,6 +71,9 @@ def _check(name: str, t: torch.Tensor, dims: int, dtypes, device: Optional[torch
 
 
 def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == device.index and t.shape == shape \
+            and t.is_contiguous() and not t.requires_grad:
+        return t
     _check(name, t, len(shape), (dtype,), device)
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)}, it is {list(t.shape)}")
@@ -117,9 +123,8 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + last * t.element_size()
 
 
-def _stream(device: torch.device) -> int:
-    """The current stream's handle, without the stream object around it."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# the current stream's handle by device index, without the stream object around it
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -133,11 +138,14 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     rows, k = x.shape
     if k > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < k:
         x = x.contiguous()
-    q = _empty_wide((rows, k), torch.int8, x.device)
-    scale = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
-    _lib.check(_lib.load().eb_quantize_rows(x.data_ptr(), rows, k, x.stride(0) if rows > 1 else k, _FLOATS[x.dtype],
-                                            q.data_ptr(), q.stride(0) if rows > 1 else k, scale.data_ptr(),
-                                            x.device.index, _stream(x.device)))
+    device, q_ld = x.device, (k + 15) // 16 * 16
+    q = torch.empty_strided((rows, k), (q_ld, 1), dtype=torch.int8, device=device)
+    scale = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device)
+    code = _lib.load().eb_quantize_rows(x.data_ptr(), rows, k, x.stride(0) if rows > 1 else k, _FLOATS[x.dtype],
+                                        q.data_ptr(), q_ld, scale.data_ptr(), device.index,
+                                        _current_stream(device.index))
+    if code:
+        _lib.check(code)
     return q, scale
 
 
@@ -151,72 +159,84 @@ def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, tor
     _check("groups", groups, 1, _INDEX)
     if not groups.is_contiguous():
         groups = groups.contiguous()
-    rows, device, lib = groups.numel(), groups.device, _lib.load()
-    need = C.c_size_t()
-    _lib.check(lib.eb_group_rows_workspace_bytes(rows, int(num_groups), C.byref(need)))
+    rows, device, lib, num_groups = groups.shape[0], groups.device, _lib.load(), int(num_groups)
     order = torch.empty_strided((rows,), (1,), dtype=torch.int32, device=device)
-    offsets = torch.empty_strided((int(num_groups) + 1,), (1,), dtype=torch.int32, device=device)
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    _lib.check(lib.eb_group_rows(groups.data_ptr(), rows, int(num_groups), _INDEX[groups.dtype], order.data_ptr(),
+    offsets = torch.empty_strided((max(0, num_groups) + 1,), (1,), dtype=torch.int32, device=device)
+    need = C.c_size_t()
+    code = lib.eb_group_rows_workspace_bytes(rows, num_groups, C.byref(need))
+    if not code:
+        ws = torch.empty_strided((need.value,), (1,), dtype=torch.uint8, device=device) if need.value else None
+        code = lib.eb_group_rows(groups.data_ptr(), rows, num_groups, _INDEX[groups.dtype], order.data_ptr(),
                                  offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, device.index,
-                                 _stream(device)))
+                                 _current_stream(device.index))
+    if code:
+        _lib.check(code)
     return order, offsets
 
 
 def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out):
     device = x.device
-    groups, n, k = weight.shape if weight.dim() == 3 else (1,) + tuple(weight.shape)
-    if activation not in _ACTIVATIONS:
+    x_rows, k = x.shape
+    if weight.dim() == 3:
+        groups, n, w_k = weight.shape
+        lead = (groups, n)
+    else:
+        n, w_k = weight.shape
+        groups, lead = 1, (n,)
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
-    if x.shape[1] != k:
-        raise ValueError(f"x has {x.shape[1]} columns, weight has {k}")
+    if k != w_k:
+        raise ValueError(f"x has {k} columns, weight has {w_k}")
     if n < 1 or k < 1 or groups < 1:
         raise ValueError(f"weight must not be empty, it is {list(weight.shape)}")
-    a = _lib.EbLinearArgs()
-    keep = []  # alive until the launch is on the stream
-    positions = x.shape[0]
+    # tensors made here stay referenced until the launch is on the stream
+    positions = x_rows
+    in_ptr = out_ptr = offsets_ptr = bias_ptr = x_scale_ptr = w_scale_ptr = 0
     if in_rows is not None:
         _check("in_rows", in_rows, 1, (torch.int32,), device)
-        keep.append(in_rows.contiguous())
-        positions, a.in_rows = in_rows.numel(), keep[-1].data_ptr()
+        in_rows = in_rows.contiguous()
+        positions, in_ptr = in_rows.shape[0], in_rows.data_ptr()
     if out_rows is not None:
         _check("out_rows", out_rows, 1, (torch.int32,), device)
-        if out_rows.numel() != positions:
-            raise ValueError(f"out_rows has {out_rows.numel()} entries for {positions} rows")
-        keep.append(out_rows.contiguous())
-        a.out_rows = keep[-1].data_ptr()
+        if out_rows.shape[0] != positions:
+            raise ValueError(f"out_rows has {out_rows.shape[0]} entries for {positions} rows")
+        out_rows = out_rows.contiguous()
+        out_ptr = out_rows.data_ptr()
     if offsets is not None:
-        keep.append(_vector("offsets", offsets, (groups + 1,), torch.int32, device))
-        a.offsets = keep[-1].data_ptr()
-    lead = (groups, n) if weight.dim() == 3 else (n,)
+        offsets = _vector("offsets", offsets, (groups + 1,), torch.int32, device)
+        offsets_ptr = offsets.data_ptr()
     if bias is not None:
-        keep.append(_vector("bias", bias, lead, torch.float32, device))
-        a.bias = keep[-1].data_ptr()
-    if x.dtype == torch.int8:
+        bias = _vector("bias", bias, lead, torch.float32, device)
+        bias_ptr = bias.data_ptr()
+    if x.dtype is torch.int8:
         if x_scale is None or weight_scale is None:
             raise ValueError("8-bit products need x_scale and weight_scale")
-        keep.append(_vector("x_scale", x_scale, (x.shape[0],), torch.float32, device))
-        a.x_scale = keep[-1].data_ptr()
-        keep.append(_vector("weight_scale", weight_scale, lead, torch.float32, device))
-        a.w_scale = keep[-1].data_ptr()
-        a.dtype = _lib.EB_ROW_I8
-        out_dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
+        x_scale = _vector("x_scale", x_scale, (x_rows,), torch.float32, device)
+        weight_scale = _vector("weight_scale", weight_scale, lead, torch.float32, device)
+        x_scale_ptr, w_scale_ptr = x_scale.data_ptr(), weight_scale.data_ptr()
+        dtype = _lib.EB_ROW_I8
+        if out_dtype is None:
+            out_dtype = torch.bfloat16 if out is None else out.dtype
     else:
         if x_scale is not None or weight_scale is not None:
             raise ValueError("scales belong to 8-bit products only")
-        if out_dtype not in (None, x.dtype):
+        if out_dtype is not None and out_dtype is not x.dtype:
             raise TypeError(f"products of {x.dtype} give {x.dtype}, not {out_dtype}")
         out_dtype = x.dtype
-        a.dtype = _FLOATS[x.dtype]
-    if out_dtype not in _FLOATS:
+        dtype = _FLOATS[out_dtype]
+    out_code = _FLOATS.get(out_dtype)
+    if out_code is None:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    zero_rest = 0
     if out is None:
         # without out_rows every position is a row of the result, and the kernel fills those of no group with zeros
         if out_rows is None:
             out = torch.empty_strided((positions, n), (n, 1), dtype=out_dtype, device=device)
-            a.zero_rest = offsets is not None
+            zero_rest = int(offsets is not None)
         else:
             out = torch.zeros((positions, n), dtype=out_dtype, device=device)
+        result_rows, out_ld = positions, n
     else:
         _check("out", out, 2, (out_dtype,), device)
         if out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
@@ -224,10 +244,13 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
         if out_rows is None and out.shape[0] < positions:
             raise ValueError(f"out has {out.shape[0]} rows for {positions}")
         lo, hi = _span(out)
-        for t in (x, weight):
-            first, last = _span(t)
-            if first < hi and lo < last:
-                raise ValueError("out must not share memory with the arguments")
+        for t in (x, weight, bias, x_scale, weight_scale, offsets, in_rows, out_rows):
+            if t is not None:
+                first, last = _span(t)
+                if first < hi and lo < last:
+                    raise ValueError("out must not share memory with the arguments")
+        result_rows = out.shape[0]
+        out_ld = out.stride(0) if result_rows > 1 else n
     x_strides, w_strides = _wide_strides(x), _wide_strides(weight)
     if x_strides is None:
         x = pack_rows(x)
@@ -235,14 +258,14 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
     if w_strides is None:
         weight = pack_rows(weight)
         w_strides = _wide_strides(weight)
-    a.x, a.weight, a.out, a.status = x.data_ptr(), weight.data_ptr(), out.data_ptr(), _status_word(device).data_ptr()
-    a.x_rows, a.x_ld = x.shape[0], x_strides[0]
-    a.w_ld, a.w_group_ld = w_strides
-    a.positions, a.out_rows_total = positions, out.shape[0]
-    a.out_ld = out.stride(0) if out.shape[0] > 1 else n
-    a.n, a.k, a.num_groups = n, k, groups
-    a.out_dtype, a.activation = _FLOATS[out_dtype], _ACTIVATIONS[activation]
-    _lib.check(_lib.load().eb_linear(C.byref(a), device.index, _stream(device)))
+    index = device.index
+    args = _lib.pack_linear_args(x.data_ptr(), weight.data_ptr(), bias_ptr, x_scale_ptr, w_scale_ptr, offsets_ptr, in_ptr,
+                                 out_ptr, out.data_ptr(), _status_word(index), x_rows, x_strides[0], w_strides[0],
+                                 w_strides[1], positions, result_rows, out_ld, n, k, groups, dtype, out_code, act,
+                                 zero_rest)
+    code = _lib.load().eb_linear(args, index, _current_stream(index))
+    if code:
+        _lib.check(code)
     return out
 
 

@@ -135,3 +135,6 @@ def test_args_struct_matches_the_header(tmp_path):
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [getattr(_lib.EbLinearArgs, n).offset for n in names] + [C.sizeof(_lib.EbLinearArgs)]
     assert np.all(np.diff(got) > 0)
+    # the packed form holds the same bytes
+    values = list(range(1, len(names) + 1))
+    assert _lib.pack_linear_args(*values) == bytes(_lib.EbLinearArgs(*values))
