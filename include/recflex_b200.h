@@ -575,7 +575,7 @@ typedef struct eb_linear_args {
 /*
  * x and weight must start on 16-byte boundaries with x_ld, w_ld and w_group_ld
  * multiples of 16 bytes (EB_ERR_UNSUPPORTED otherwise).  At most 2^31 - 1025
- * positions and rows, and 2^30 columns.
+ * positions and rows, and 2^30 columns and units.
  */
 int eb_linear(const eb_linear_args* args, int device, void* stream);
 

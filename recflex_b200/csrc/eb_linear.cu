@@ -3,7 +3,7 @@
 // rows summed in 32-bit integers.
 //
 // A CTA (or a pair of CTAs on neighbouring SMs) walks output tiles of
-// 128 (256) rows x BN columns: one warp copies the operands into a ring of
+// 128 (256) rows x BN columns: a few threads copy the operands into a ring of
 // shared-memory stages of 128 bytes of K (tensor copies; rows taken by index go
 // through the four-row gather form, so no reordered copy of x is ever made), one
 // thread issues tcgen05 products into one of two accumulators in tensor memory,
@@ -11,6 +11,13 @@
 // activation and the rounding in registers, then through shared memory so that
 // whole row segments are stored, wherever their rows go.  Which tiles there are
 // follows from the offsets on the GPU; the host never reads them.
+//
+// What bounds it: the tensor units for long K (int8 16384 x 15608 x 1024 in
+// 0.169 ms, 3.1 Pop/s; bf16 of that size in 8 groups, rows by index, 0.395 ms,
+// 1.33 Pflop/s), and before them the way of the operands from L2 to the SMs,
+// about 55 bytes a clock and SM, which is why the widest tile wins there; for
+// short K the way from launch to the first products and from the last to the
+// stored results, about 8 us of int8 4096 x 1924 x 1024's 13.8.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -212,8 +219,13 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
   }
 }
 
-// SPLIT: the CTAs of a cluster share a tile and take a piece of K each (all warps meet at two cluster barriers a tile, also when one gave up); their accumulators are added through
-// distributed shared memory in the order of their ranks, so that the result is the same on every run.  (With CG = 1.)
+// CG = 2: a pair of CTAs shares a tile of 256 rows; each copies its 128 rows of x and its half of the weights' rows, the
+// first one's thread issues the products of both, and each stores its rows.  The pair halves the weights' way from L2.
+// SPLIT (CG = 1): the CTAs of a cluster share a tile and take a piece of K each; their accumulators are added through
+// distributed shared memory in the order of their ranks, so that the result is the same on every run.  All warps meet
+// at two cluster barriers a tile, also when one gave up.
+// Every wait ends: after two seconds a thread gives up, sets a bit of the status word, and the CTA drains what is under
+// way and returns.
 template <bool I8, int BN, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     eb_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ CUtensorMap map_x,
@@ -756,7 +768,7 @@ int eb_linear(const eb_linear_args* args, int device, void* stream) {
   if (a.n < 1 || a.k < 1 || a.num_groups < 1 || a.positions < 0 || a.x_rows < 0 || a.out_rows_total < 0)
     return linear_fail(EB_ERR_INVALID_ARG, "bad size: n %d, k %d, num_groups %d", a.n, a.k, a.num_groups);
   if (a.num_groups > EB_MAX_GROUPS) return linear_fail(EB_ERR_TOO_LARGE, "%d groups, at most %d", a.num_groups, EB_MAX_GROUPS);
-  if (a.k > (1 << 30)) return linear_fail(EB_ERR_TOO_LARGE, "%d columns, at most 2^30", a.k);
+  if (a.k > (1 << 30) || a.n > (1 << 30)) return linear_fail(EB_ERR_TOO_LARGE, "%d x %d columns, at most 2^30", a.k, a.n);
   if (i8 && a.k > EB_MAX_I8_COLS) return linear_fail(EB_ERR_TOO_LARGE, "%d columns of 8 bits, at most %d", a.k, EB_MAX_I8_COLS);
   if (a.positions > kMaxRows || a.x_rows > kMaxRows || a.out_rows_total > kMaxRows)
     return linear_fail(EB_ERR_TOO_LARGE, "more than %lld rows", (long long)kMaxRows);

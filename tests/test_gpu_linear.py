@@ -157,6 +157,56 @@ def test_int8_linear_large(rows, k, n):
     assert torch.equal(out, again)
 
 
+# sizes that reach each of the tiles (512 and 256 columns on pairs of CTAs, 256, 128, 64 and 16 columns on one, K split
+# over two and four), with columns and K that end inside them
+TILES = [(16384, 15608, 1024), (16300, 15000, 1001), (9000, 6000, 1000), (4096, 1924, 333), (4096, 480, 1000),
+         (2000, 1924, 777), (1000, 1030, 65), (5000, 3001, 15), (512, 15608, 700), (333, 9001, 300)]
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows, k, n", TILES)
+def test_int8_linear_on_every_tile(rows, k, n, dtype, act):
+    if rows * k > 1 << 26 and (dtype, act) not in ((torch.float32, "sigmoid"), (torch.bfloat16, "relu"), (torch.float16, "none")):
+        pytest.skip("the largest sizes run once for each type and activation")
+    g = gen(rows + k + n)
+    q, w = codes((rows, k), g), codes((n, k), g)
+    # results of a few units, where the sigmoid bends
+    qs = scales(rows, g) * 8 / k ** 0.5
+    ws, bias = scales(n, g), torch.randn(n, generator=g, device=DEV)
+    wide = torch.full((rows + 1, n + 3), 7.0, dtype=dtype, device=DEV)
+    out = linear.int8_linear(q, qs, w, ws, bias, act, dtype)
+    check_int8(q, qs, w, ws, bias, act, out)
+    linear.int8_linear(q, qs, w, ws, bias, act, dtype, out=wide[:, 1:n + 1])  # rows that take no wide stores
+    assert torch.equal(wide[:rows, 1:n + 1], out)
+    assert (wide[:, 0] == 7).all() and (wide[:, n + 1:] == 7).all() and (wide[rows] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "i8"])
+@pytest.mark.parametrize("rows, groups, k, n", [(9000, 9, 1924, 500), (9000, 9, 1924, 1000), (12000, 9, 1924, 1000),
+                                                (20000, 9, 1030, 250), (3000, 40, 1924, 1000), (700, 3, 9000, 300)])
+@pytest.mark.parametrize("gather", [False, True])
+def test_grouped_linear_on_every_tile(rows, groups, k, n, kind, gather):
+    g = gen(rows + groups + n)
+    ids = torch.randint(-1, groups, (rows,), generator=g, device=DEV) * torch.randint(0, 2, (rows,), generator=g, device=DEV)
+    order, offsets = linear.group_rows(ids, groups)
+    kw = {}
+    if kind == "i8":
+        x, w = codes((rows, k), g), codes((groups, n, k), g)
+        kw = dict(x_scale=scales(rows, g), weight_scale=scales(groups * n, g).view(groups, n))
+    else:
+        dtype = torch.bfloat16 if kind == "bf16" else torch.float16
+        x = torch.randn(rows, k, generator=g, device=DEV).to(dtype)
+        w = (torch.randn(groups, n, k, generator=g, device=DEV) / k ** 0.5).to(dtype)
+    bias = torch.randn(groups, n, generator=g, device=DEV)
+    rows_in = order if gather else None
+    got = linear.grouped_linear(x, w, offsets, bias, "relu", rows_in, order, **kw)
+    exact, slack = plain_grouped(x, w, offsets, bias, "relu", rows_in, order, torch.zeros_like(got), kw.get("x_scale"), kw.get("weight_scale"))
+    check(got, exact, slack)
+    assert torch.equal(got, linear.grouped_linear(x, w, offsets, bias, "relu", rows_in, order, **kw))
+    linear.check_status(DEV)
+
+
 def test_int8_linear_layouts_and_given_out():
     g = gen(3)
     base, wbase = codes((64, 300), g), codes((50, 400), g)
@@ -385,6 +435,48 @@ def test_bad_rows_and_offsets_are_reported_and_skipped():
         same = linear.grouped_linear(x, w, torch.tensor(clamped, dtype=torch.int32, device=DEV))
         assert torch.equal(out, same)
         reported()
+
+
+def test_far_offsets():
+    """Rows, weights and results that lie behind 2^31 elements."""
+    g = gen(40)
+    x = torch.empty(140000, 16000, dtype=torch.float16, device=DEV)
+    for part in x.split(20000):
+        part.normal_(generator=g)
+    q, scale = linear.quantize_rows(x)
+    for at in (slice(0, 3), slice(139990, 140000)):
+        check_codes(x[at], q[at], scale[at])
+    del x
+    w = codes((40, 16000), g)
+    ws = scales(40, g)
+    out = linear.int8_linear(q, scale, w, ws, out_dtype=torch.float32)
+    check_int8(q[-300:], scale[-300:], w, ws, None, "none", out[-300:])
+    last = torch.arange(139999, 139000, -1, dtype=torch.int32, device=DEV)
+    part = linear.grouped_linear(q, w[None], offsets_of([1000]), in_rows=last, x_scale=scale, weight_scale=ws[None], out_dtype=torch.float32)
+    assert torch.equal(part, out[last.long()])
+    few = linear.grouped_linear(q, w[None], offsets_of([3]), in_rows=last[:3].contiguous(), x_scale=scale, weight_scale=ws[None], out_dtype=torch.float32)
+    assert torch.equal(few, part[:3])  # sums of whole numbers: the same from every kernel
+    del q, out
+    rows, n = 2200000, 1000
+    q, w = codes((rows, 16), g), codes((n, 16), g)
+    qs, ws = scales(rows, g), scales(n, g)
+    out = linear.int8_linear(q, qs, w, ws)
+    for at in (slice(0, 200), slice(rows - 200, rows)):
+        check_int8(q[at], qs[at], w, ws, None, "none", out[at])
+    back = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device=DEV)
+    turned = linear.grouped_linear(q, w[None], offsets_of([rows]), out_rows=back, x_scale=qs, weight_scale=ws[None], out=torch.empty_like(out))
+    assert torch.equal(turned[0], out[-1]) and torch.equal(turned[-1], out[0]) and torch.equal(turned[rows // 2], out[rows - 1 - rows // 2])
+    del out, turned, q
+    w = torch.empty(70, 1000, 32000, dtype=torch.float16, device=DEV)
+    for part in w.split(10):
+        part.normal_(generator=g)
+    x = torch.randn(900, 32000, generator=g, device=DEV).half()
+    for sizes in ([0] * 66 + [1, 0, 1, 1], [0] * 66 + [100, 0, 200, 600]):  # a few rows, and tiles
+        offsets = offsets_of(sizes)
+        got = linear.grouped_linear(x[:sum(sizes)], w, offsets)
+        exact, slack = plain_grouped(x[:sum(sizes)], w, offsets, None, "none", None, None, torch.zeros_like(got))
+        check(got, exact, slack)
+    linear.check_status(DEV)
 
 
 # ---- refusals ----------------------------------------------------------------------------------------------------

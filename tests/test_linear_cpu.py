@@ -72,6 +72,8 @@ def product(lib, **kw):
     (dict(n=0), _lib.EB_ERR_INVALID_ARG), (dict(k=0), _lib.EB_ERR_INVALID_ARG),
     (dict(num_groups=0), _lib.EB_ERR_INVALID_ARG), (dict(num_groups=_lib.EB_MAX_GROUPS + 1), _lib.EB_ERR_TOO_LARGE),
     (dict(k=_lib.EB_MAX_I8_COLS + 1), _lib.EB_ERR_TOO_LARGE), (dict(positions=1 << 31), _lib.EB_ERR_TOO_LARGE),
+    (dict(n=(1 << 30) + 1), _lib.EB_ERR_TOO_LARGE), (dict(positions=(1 << 31) - 1024), _lib.EB_ERR_TOO_LARGE),
+    (dict(dtype=_lib.EB_OUT_F16, out_dtype=_lib.EB_OUT_F16, k=(1 << 30) + 1), _lib.EB_ERR_TOO_LARGE),
     (dict(positions=-1), _lib.EB_ERR_INVALID_ARG), (dict(offsets=None), _lib.EB_ERR_INVALID_ARG),
     (dict(positions=9), _lib.EB_ERR_INVALID_ARG), (dict(out_rows_total=7), _lib.EB_ERR_INVALID_ARG),
     (dict(x=None), _lib.EB_ERR_INVALID_ARG), (dict(weight=None), _lib.EB_ERR_INVALID_ARG),
