@@ -452,7 +452,7 @@ def test_far_offsets():
     out = linear.int8_linear(q, scale, w, ws, out_dtype=torch.float32)
     check_int8(q[-300:], scale[-300:], w, ws, None, "none", out[-300:])
     last = torch.arange(139999, 139000, -1, dtype=torch.int32, device=DEV)
-    part = linear.grouped_linear(q, w[None], offsets_of([1000]), in_rows=last, x_scale=scale, weight_scale=ws[None], out_dtype=torch.float32)
+    part = linear.grouped_linear(q, w[None], offsets_of([last.numel()]), in_rows=last, x_scale=scale, weight_scale=ws[None], out_dtype=torch.float32)
     assert torch.equal(part, out[last.long()])
     few = linear.grouped_linear(q, w[None], offsets_of([3]), in_rows=last[:3].contiguous(), x_scale=scale, weight_scale=ws[None], out_dtype=torch.float32)
     assert torch.equal(few, part[:3])  # sums of whole numbers: the same from every kernel
