@@ -56,7 +56,7 @@ struct Shape {
   static constexpr int kPart = BN / kParts;
   static constexpr int kWRows = kPart / CG;  // rows of the weight that one CTA of a pair copies for a part
   static constexpr int kStageBytes = kABytes + kParts * kWRows * kKBytes;
-  static constexpr int kStagingRow = kParts > 1 ? 64 : 128;  // bytes of a result row that are stored at once
+  static constexpr int kStagingRow = kParts > 1 || kPart <= 64 ? 64 : 128;  // bytes of a result row that are stored at once
   static constexpr int kStaging = 32 * kStagingRow;          // per storing warp
   static constexpr int kFixed = 1024 /* alignment */ + kEpilogueWarps * (kStaging + kColumnBytes) + 256 /* barriers */ +
                                 2 * 4 * (EB_MAX_GROUPS + 1) + 8;
@@ -70,6 +70,7 @@ struct LinearArgs {
   int n_tiles, k_steps;
   int cluster;  // CTAs of a cluster: CG, or the number of pieces that K is split into
   int wide;     // rows of out take 16-byte stores
+  int boxes;    // results go out in boxes of 32 rows (map_out), where a warp has that many: rows in order, `wide`
 };
 
 struct Tile {
@@ -131,9 +132,10 @@ __device__ __forceinline__ void shared_write(uint32_t at, uint32_t a, uint32_t b
 // ways.  relu is a maximum with a bound of 0 or -infinity.  What this costs is instructions (two warps share a scheduler,
 // 64 columns each at a time): 14 a value, with a bound and a branch for each, took 2000 clocks per 64 columns; pairs of
 // fp32 operations, the bound on packed pairs and a path of its own for the sigmoid leave about 5.
-template <bool I8, int OUT, bool SIGMOID, int SPAN, int ROWB>
-__device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, const RowInfo& r, const float* scales,
-                                           const float* biases, int n, uint32_t mine, int lane) {
+template <bool I8, int OUT, bool SIGMOID, bool BOX, int SPAN, int ROWB>
+__device__ __forceinline__ void store_span(const LinearArgs& args, const CUtensorMap* map_out, uint32_t tm, const RowInfo& r,
+                                           const float* scales, const float* biases, int n, int first_row,
+                                           uint32_t mine, int lane) {
   const eb_linear_args& a = args.a;
   constexpr int kSize = OUT == EB_OUT_F32 ? 4 : 2, kElems = 16 / kSize;
   constexpr int kUnit = SPAN < ROWB / kSize ? SPAN : ROWB / kSize, kLoad = kUnit < 32 ? kUnit : 32;
@@ -146,15 +148,18 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
   const bool any_zero = !I8 && __any_sync(0xffffffffu, r.zero);
   const float2 row_scale = make_float2(r.scale, r.scale);
   const int piece = lane % kPieces;
-  uint8_t* to[kPieces];  // this lane's rows
+  uint8_t* to[BOX ? 1 : kPieces];  // this lane's rows
+  if constexpr (!BOX) {
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int dst = __shfl_sync(0xffffffffu, r.dst, i * kRowsOnce + lane / kPieces);
-    to[i] = dst < 0 ? nullptr : static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + n) * kSize + piece * 16;
+    for (int i = 0; i < kPieces; ++i) {
+      const int dst = __shfl_sync(0xffffffffu, r.dst, i * kRowsOnce + lane / kPieces);
+      to[i] = dst < 0 ? nullptr : static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + n) * kSize + piece * 16;
+    }
   }
 #pragma unroll 1
   for (int c = 0; c < SPAN && n + c < a.n; c += kUnit) {
     uint32_t v[kLoad];
+    if (elect_one()) store_wait_read();
     __syncwarp();  // the unit before has been read
 #pragma unroll
     for (int i = 0; i < kUnit; i += 8) {
@@ -190,7 +195,12 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
         shared_write(mine + place(lane, i / 8), pack2<OUT>(o[0], low2), pack2<OUT>(o[1], low2), pack2<OUT>(o[2], low2), pack2<OUT>(o[3], low2));
       }
     }
-    __syncwarp();
+    if constexpr (BOX) {
+      fence_copies();
+      __syncwarp();
+      if (elect_one()) store_2d(map_out, n + c, first_row, mine);
+    } else {
+      __syncwarp();
     const bool whole = args.wide && n + c + kUnit <= a.n;
     uint4 out[kPieces];
 #pragma unroll
@@ -216,6 +226,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
         }
       }
     }
+    }
   }
 }
 
@@ -229,7 +240,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, uint32_t tm, 
 template <bool I8, int BN, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     eb_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ CUtensorMap map_x,
-                     const __grid_constant__ CUtensorMap map_w) {
+                     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
   using S = Shape<BN, CG>;
   static_assert(!SPLIT || CG == 1, "a pair of CTAs shares its tile already");
   constexpr int kStages = S::kStages;
@@ -289,15 +300,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int pieces = SPLIT ? args.cluster : 1;
   const int k_first = SPLIT ? (int)((int64_t)args.k_steps * rank / pieces) : 0;
   const int k_last = SPLIT ? (int)((int64_t)args.k_steps * (rank + 1) / pieces) : args.k_steps;
-  const int64_t total = (int64_t)tiles[a.num_groups] * args.n_tiles;
-  const int64_t stride = gridDim.x / args.cluster;
-  auto tile_at = [&](int64_t t) {
+  // The tiles of this CTA (cluster), columns innermost, without a division or a search for each: those cost every role 400
+  // to 800 clocks a tile.
+  const int clusters = gridDim.x / args.cluster;
+  const int m_step = clusters / args.n_tiles, n_step = clusters % args.n_tiles, m_tiles = tiles[a.num_groups];
+  struct Walk {
+    int mt, nt, group;
+  };
+  auto first_tile = [&] {
+    const int t = blockIdx.x / args.cluster;
+    return Walk{t / args.n_tiles, t % args.n_tiles, 0};
+  };
+  auto advance = [&](Walk& w) {
+    w.mt += m_step;
+    w.nt += n_step;
+    if (w.nt >= args.n_tiles) {
+      w.nt -= args.n_tiles;
+      ++w.mt;
+    }
+  };
+  auto tile_at = [&](Walk& w) {  // w.mt < m_tiles
+    while (tiles[w.group + 1] <= w.mt) ++w.group;
     Tile r;
-    const int mt = (int)(t / args.n_tiles);
-    r.group = find_group(tiles, a.num_groups, mt);
-    r.m0 = off[r.group] + (mt - tiles[r.group]) * S::kRows;
+    r.group = w.group;
+    r.m0 = off[r.group] + (w.mt - tiles[r.group]) * S::kRows;
     r.m1 = off[r.group + 1];
-    r.n0 = (int)(t % args.n_tiles) * BN;
+    r.n0 = w.nt * BN;
     return r;
   };
   auto rows_of = [&](const Tile& t, uint32_t r) { return min(max(t.m1 - t.m0 - (CG > 1 ? 128 * (int)r : 0), 0), 128); };
@@ -309,9 +337,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kQuads = (32 + kCopyWarps - 1) / kCopyWarps;
     bool ok = true;
     uint32_t st = 0, phase = 1;
-    for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride) {
+    for (Walk walk = first_tile(); walk.mt < m_tiles && (ok || SPLIT); advance(walk)) {
       if (warp < copiers && elect_one()) {
-        const Tile tile = tile_at(t);
+        const Tile tile = tile_at(walk);
         const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0), rows = rows_of(tile, rank);
         const int quads = max(0, ((rows + 3) / 4 - warp + kCopyWarps - 1) / kCopyWarps);  // of this warp
         const bool box = kBoxRows * warp < rows;
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kKBytes / 32; ++i) multiply<I8, CG>(tmem + slot * S::kPart, x + 2 * i, w + 2 * i, desc, add || i > 0);
     };
-    for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride, ++count) {
+    for (Walk walk = first_tile(); walk.mt < m_tiles && (ok || SPLIT); advance(walk), ++count) {
       if (leader && elect_one()) {
         const int steps = k_last - k_first;
         if constexpr (S::kParts == 1) {
@@ -456,13 +484,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kColumnsEach = S::kPart >= 64 ? S::kPart / 64 : 1;
     RowInfo next_row{-1, 0.0f, false};
     float next_scale[kColumnsEach], next_bias[kColumnsEach];
-    auto fetch_row = [&](int64_t t) {
-      const Tile tile = tile_at(t);
+    auto fetch_row = [&](const Tile& tile) {
       const int p = tile.m0 + (CG > 1 ? 128 * (int)rank : 0) + quad * 32 + lane;
       next_row = row_info<I8>(a, p, S::kPart >= 64 || half == 0 ? tile.m1 : 0);
     };
-    auto fetch_columns = [&](int64_t t, int part) {
-      const Tile tile = tile_at(t);
+    auto fetch_columns = [&](const Tile& tile, int part) {
       const int n = tile.n0 + part * S::kPart + (S::kPart >= 64 ? half * (S::kPart / 2) : 0) + lane;
       const int64_t at = (int64_t)tile.group * a.n + n;
 #pragma unroll
@@ -474,8 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     bool ok = true;
     uint32_t count = 0;
-    for (int64_t t = blockIdx.x / args.cluster; t < total && (ok || SPLIT); t += stride, ++count) {
-      const Tile tile = tile_at(t);
+    Walk walk = first_tile();
+    Tile next_tile{};
+    if (walk.mt < m_tiles) next_tile = tile_at(walk);
+    while (walk.mt < m_tiles && (ok || SPLIT)) {
+      const Tile tile = next_tile;
+      advance(walk);
+      const bool more = walk.mt < m_tiles;
+      if (more) next_tile = tile_at(walk);
       const int m_cta = tile.m0 + (CG > 1 ? 128 * (int)rank : 0);
       const int rows = rows_of(tile, rank);
       if constexpr (!SPLIT) {
@@ -484,8 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kEach = (kSpan + 31) / 32;
         const bool work = half < kHalves && quad * 32 < rows;
         if (count == 0) {
-          fetch_row(t);
-          fetch_columns(t, 0);
+          fetch_row(tile);
+          fetch_columns(tile, 0);
         }
         const RowInfo r = next_row;
 #pragma unroll 1
@@ -506,21 +538,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_after();
           // on their way while this part is stored
           if (part + 1 < S::kParts) {
-            fetch_columns(t, part + 1);
-          } else if (t + stride < total) {
-            fetch_row(t + stride);
-            fetch_columns(t + stride, 0);
+            fetch_columns(tile, part + 1);
+          } else if (more) {
+            fetch_row(next_tile);
+            fetch_columns(next_tile, 0);
           }
           if (work) {
             const uint32_t tm = tmem + slot * S::kPart + half * kSpan + ((uint32_t)(quad * 32) << 16);
-            auto store = [&](auto out, auto sigmoid) {
-              store_span<I8, decltype(out)::value, decltype(sigmoid)::value, kSpan, S::kStagingRow>(args, tm, r, col_scale, col_bias, n, mine, lane);
+            const bool box = args.boxes && rows - quad * 32 >= 32;
+            auto store = [&](auto out, auto sigmoid, auto box) {
+              store_span<I8, decltype(out)::value, decltype(sigmoid)::value, decltype(box)::value, kSpan, S::kStagingRow>(
+                  args, &map_out, tm, r, col_scale, col_bias, n, m_cta + quad * 32, mine, lane);
             };
             auto store_as = [&](auto out) {
               if (a.activation == EB_ACT_SIGMOID)
-                store(out, std::true_type{});
+                box ? store(out, std::true_type{}, std::true_type{}) : store(out, std::true_type{}, std::false_type{});
               else
-                store(out, std::false_type{});
+                box ? store(out, std::false_type{}, std::true_type{}) : store(out, std::false_type{}, std::false_type{});
             };
             if (a.out_dtype == EB_OUT_BF16)
               store_as(std::integral_constant<int, EB_OUT_BF16>{});
@@ -592,10 +626,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the next tile's copies write where these sums were read
         __syncwarp();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_copies();
         cluster_sync();
       }
+      ++count;
     }
+    if (!SPLIT && elect_one()) store_wait_read();
   }
 
   __syncwarp();
@@ -638,19 +674,21 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// A [groups, rows, k] tensor of `dtype` read in boxes of `box_rows` rows x 128 bytes; what lies outside reads as zeros.
+// A [groups, rows, k] tensor of `dtype` in boxes of `box_rows` rows x `box_bytes` (128 or 64, swizzled as wide); what lies
+// outside reads as zeros and is not written.
 bool make_map(CUtensorMap* map, int dims, int dtype, const void* p, int64_t k, int64_t rows, int64_t ld, int64_t groups,
-              int64_t group_ld, int box_rows) {
-  const int size = dtype == EB_ROW_I8 ? 1 : 2;
+              int64_t group_ld, int box_rows, int box_bytes = kKBytes) {
+  const int size = dtype == EB_ROW_I8 ? 1 : dtype == EB_OUT_F32 ? 4 : 2;
   const CUtensorMapDataType type = dtype == EB_ROW_I8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == EB_OUT_F32  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == EB_OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint64_t extent[3] = {(cuuint64_t)k, (cuuint64_t)rows, (cuuint64_t)groups};
   const cuuint64_t pitch[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(group_ld * size)};
-  const cuuint32_t box[3] = {(cuuint32_t)(kKBytes / size), (cuuint32_t)box_rows, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)(box_bytes / size), (cuuint32_t)box_rows, 1};
   const cuuint32_t step[3] = {1, 1, 1};
   return encode_tiled()(map, type, dims, const_cast<void*>(p), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -662,13 +700,18 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   const eb_linear_args& a = args.a;
   args.n_tiles = (a.n + BN - 1) / BN;
   args.cluster = SPLIT ? split : CG;
-  CUtensorMap map_x, map_w;
+  CUtensorMap map_x, map_w, map_out = {};
   // rows of x that are all out of range are never used: any memory of the right length will do
   const void* x = a.x_rows ? a.x : a.weight;
   if (!make_map(&map_x, 2, a.dtype, x, a.k, a.x_rows ? a.x_rows : 1, a.x_ld, 1, 0, a.in_rows ? 1 : kBoxRows) ||
       !make_map(&map_w, 3, a.dtype, a.weight, a.k, a.n, a.w_ld, a.num_groups, a.w_group_ld, S::kWRows))
     return linear_fail(EB_ERR_INVALID_ARG, "the driver refused a tensor map for %d x %d of pitch %lld / %lld", a.n, a.k,
                        (long long)a.x_ld, (long long)a.w_ld);
+  // a unit of columns of 32 rows; tiles whose unit is narrower than a staging row store row by row
+  constexpr int kSpan = S::kPart >= 64 ? S::kPart / 2 : S::kPart;
+  const int size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
+  args.boxes = !SPLIT && args.wide && !a.out_rows && kSpan * size >= S::kStagingRow &&
+               make_map(&map_out, 2, a.out_dtype, a.out, a.n, a.out_rows_total, a.out_ld, 1, 0, 32, S::kStagingRow);
   const auto kernel = eb_linear_kernel<I8, BN, CG, SPLIT>;
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel may use this much shared memory
   if (!(ready.load() >> device & 1)) {
@@ -689,7 +732,7 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   attr[0].val.clusterDim = {(unsigned)args.cluster, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = args.cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args, map_x, map_w);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args, map_x, map_w, map_out);
   if (e != cudaSuccess) return linear_fail(EB_ERR_CUDA, "eb_linear: %s", cudaGetErrorString(e));
   return EB_OK;
 }
