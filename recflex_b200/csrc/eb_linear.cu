@@ -43,6 +43,7 @@ constexpr int kThreads = kFirstEpilogue + 32 * kEpilogueWarps;
 constexpr int kKBytes = 128;                        // K of one stage: a row of the 128-byte swizzle
 constexpr int kABytes = 128 * kKBytes;
 constexpr int kBoxRows = 128 / kBoxWarps;           // rows of x per tensor copy: a ragged tile copies only its own boxes
+constexpr int kStagingRow = 64;                     // bytes of a result row that are stored at once
 constexpr int kColumnBytes = 1024;                  // per storing warp: scale and bias of its 128 columns
 constexpr int kSmemMax = 232448;
 constexpr int kMaxSplit = 4;                        // pieces of K (clusters of 8 such CTAs do not fill the SMs)
@@ -56,8 +57,8 @@ struct Shape {
   static constexpr int kPart = BN / kParts;
   static constexpr int kWRows = kPart / CG;  // rows of the weight that one CTA of a pair copies for a part
   static constexpr int kStageBytes = kABytes + kParts * kWRows * kKBytes;
-  static constexpr int kStagingRow = kParts > 1 || kPart <= 64 ? 64 : 128;  // bytes of a result row that are stored at once
-  static constexpr int kStaging = 32 * kStagingRow;          // per storing warp
+  static constexpr int kBuffers = kParts > 1 ? 1 : 2;  // of results on their way out, per storing warp
+  static constexpr int kStaging = kBuffers * 32 * kStagingRow;
   static constexpr int kFixed = 1024 /* alignment */ + kEpilogueWarps * (kStaging + kColumnBytes) + 256 /* barriers */ +
                                 2 * 4 * (EB_MAX_GROUPS + 1) + 8;
   static constexpr int kStages = (kSmemMax - kFixed) / kStageBytes > 10 ? 10 : (kSmemMax - kFixed) / kStageBytes;
@@ -132,17 +133,15 @@ __device__ __forceinline__ void shared_write(uint32_t at, uint32_t a, uint32_t b
 // ways.  relu is a maximum with a bound of 0 or -infinity.  What this costs is instructions (two warps share a scheduler,
 // 64 columns each at a time): 14 a value, with a bound and a branch for each, took 2000 clocks per 64 columns; pairs of
 // fp32 operations, the bound on packed pairs and a path of its own for the sigmoid leave about 5.
-template <bool I8, int OUT, bool SIGMOID, bool BOX, int SPAN, int ROWB>
+template <bool I8, int OUT, bool SIGMOID, bool BOX, int SPAN, int BUFFERS>
 __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtensorMap* map_out, uint32_t tm, const RowInfo& r,
                                            const float* scales, const float* biases, int n, int first_row,
-                                           uint32_t mine, int lane) {
+                                           uint32_t staging, uint32_t& buffer, int lane) {
   const eb_linear_args& a = args.a;
   constexpr int kSize = OUT == EB_OUT_F32 ? 4 : 2, kElems = 16 / kSize;
-  constexpr int kUnit = SPAN < ROWB / kSize ? SPAN : ROWB / kSize, kLoad = kUnit < 32 ? kUnit : 32;
+  constexpr int kUnit = SPAN < kStagingRow / kSize ? SPAN : kStagingRow / kSize;
   constexpr int kPieces = kUnit / kElems, kRowsOnce = 32 / kPieces;
-  auto place = [](int row, int piece) {
-    return row * ROWB + ((ROWB == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4);
-  };
+  auto place = [](int row, int piece) { return row * kStagingRow + ((piece ^ ((row >> 1) & 3)) << 4); };
   const float low = a.activation == EB_ACT_RELU ? 0.0f : __int_as_float(0xff800000);
   const uint32_t low2 = a.activation == EB_ACT_RELU ? 0u : OUT == EB_OUT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
   const bool any_zero = !I8 && __any_sync(0xffffffffu, r.zero);
@@ -158,19 +157,18 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
   }
 #pragma unroll 1
   for (int c = 0; c < SPAN && n + c < a.n; c += kUnit) {
-    uint32_t v[kLoad];
-    if (elect_one()) store_wait_read();
-    __syncwarp();  // the unit before has been read
+    uint32_t v[kUnit];
+    tmem_load(tm + c, v);
+    if (elect_one()) store_wait_read<BUFFERS - 1>();
+    __syncwarp();  // this buffer's results have been read
+    const uint32_t mine = staging + buffer;
+    tmem_wait_load();
+    if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
+#pragma unroll
+      for (int j = 0; j < kUnit; ++j) v[j] = 0;
+    }
 #pragma unroll
     for (int i = 0; i < kUnit; i += 8) {
-      if (i % kLoad == 0) {
-        tmem_load(tm + c + i, v);
-        tmem_wait_load();
-        if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
-#pragma unroll
-          for (int j = 0; j < kLoad; ++j) v[j] = 0;
-        }
-      }
       float2 o[4], f[4], b[4];
       *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(biases + c + i);
       *reinterpret_cast<float4*>(b + 2) = *reinterpret_cast<const float4*>(biases + c + i + 4);
@@ -180,7 +178,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t x = v[i % kLoad + 2 * j], y = v[i % kLoad + 2 * j + 1];
+        const uint32_t x = v[i + 2 * j], y = v[i + 2 * j + 1];
         if constexpr (I8)
           o[j] = fma2(make_float2((float)(int)x, (float)(int)y), mul2(row_scale, f[j]), b[j]);
         else
@@ -199,6 +197,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
       fence_copies();
       __syncwarp();
       if (elect_one()) store_2d(map_out, n + c, first_row, mine);
+      if (BUFFERS > 1) buffer ^= 32 * kStagingRow;
     } else {
       __syncwarp();
     const bool whole = args.wide && n + c + kUnit <= a.n;
@@ -475,6 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int e = warp - kCopyWarps - 1, quad = warp % 4, half = e / 4;
     const uint32_t mine = staging + e * S::kStaging;
+    uint32_t buffer = 0;  // of the two that take turns, where there are two
     float* col_scale = columns + e * (kColumnBytes / 4);
     float* col_bias = col_scale + 128;
     if (a.zero_rest)
@@ -547,8 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t tm = tmem + slot * S::kPart + half * kSpan + ((uint32_t)(quad * 32) << 16);
             const bool box = args.boxes && rows - quad * 32 >= 32;
             auto store = [&](auto out, auto sigmoid, auto box) {
-              store_span<I8, decltype(out)::value, decltype(sigmoid)::value, decltype(box)::value, kSpan, S::kStagingRow>(
-                  args, &map_out, tm, r, col_scale, col_bias, n, m_cta + quad * 32, mine, lane);
+              store_span<I8, decltype(out)::value, decltype(sigmoid)::value, decltype(box)::value, kSpan, S::kBuffers>(
+                  args, &map_out, tm, r, col_scale, col_bias, n, m_cta + quad * 32, mine, buffer, lane);
             };
             auto store_as = [&](auto out) {
               if (a.activation == EB_ACT_SIGMOID)
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ++count;
     }
-    if (!SPLIT && elect_one()) store_wait_read();
+    if (!SPLIT && elect_one()) store_wait_read<0>();
   }
 
   __syncwarp();
@@ -710,8 +710,8 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   // a unit of columns of 32 rows; tiles whose unit is narrower than a staging row store row by row
   constexpr int kSpan = S::kPart >= 64 ? S::kPart / 2 : S::kPart;
   const int size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
-  args.boxes = !SPLIT && args.wide && !a.out_rows && kSpan * size >= S::kStagingRow &&
-               make_map(&map_out, 2, a.out_dtype, a.out, a.n, a.out_rows_total, a.out_ld, 1, 0, 32, S::kStagingRow);
+  args.boxes = !SPLIT && args.wide && !a.out_rows && kSpan * size >= kStagingRow &&
+               make_map(&map_out, 2, a.out_dtype, a.out, a.n, a.out_rows_total, a.out_ld, 1, 0, 32, kStagingRow);
   const auto kernel = eb_linear_kernel<I8, BN, CG, SPLIT>;
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel may use this much shared memory
   if (!(ready.load() >> device & 1)) {

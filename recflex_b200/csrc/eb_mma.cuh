@@ -134,8 +134,11 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, u
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// This thread's stores so far have read their shared memory.
-__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// All but the last LEFT of this thread's stores have read their shared memory.
+template <int LEFT>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
 
 // ---- tensor memory ---------------------------------------------------------
 template <int CG>
