@@ -70,8 +70,8 @@ struct LinearArgs {
   eb_linear_args a;
   int n_tiles, k_steps;
   int cluster;  // CTAs of a cluster: CG, or the number of pieces that K is split into
-  int wide;     // rows of out take 16-byte stores
-  int boxes;    // results go out in boxes of 32 rows (map_out), where a warp has that many: rows in order, `wide`
+  int align;    // rows of out start on multiples of 16, 4 or 2 bytes
+  int boxes;    // results go out in boxes of 32 rows (map_out), where a warp has that many: rows in order, align 16
 };
 
 struct Tile {
@@ -200,31 +200,54 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
       if (BUFFERS > 1) buffer ^= 32 * kStagingRow;
     } else {
       __syncwarp();
-    const bool whole = args.wide && n + c + kUnit <= a.n;
-    uint4 out[kPieces];
+      if (args.align == 16 || SPAN < 32) {
+        const bool whole = args.align == 16 && n + c + kUnit <= a.n;
+        uint4 out[kPieces];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) out[i] = shared_read(mine + place(i * kRowsOnce + lane / kPieces, piece));
+        for (int i = 0; i < kPieces; ++i) out[i] = shared_read(mine + place(i * kRowsOnce + lane / kPieces, piece));
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const uint4 w = out[i];
-      uint8_t* at = to[i] + c * kSize;
-      if (!to[i]) continue;
-      if (whole) {
-        *reinterpret_cast<uint4*>(at) = w;
-        continue;
-      }
-      const int left = a.n - (n + c + piece * kElems);
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        for (int i = 0; i < kPieces; ++i) {
+          const uint4 w = out[i];
+          uint8_t* at = to[i] + c * kSize;
+          if (!to[i]) continue;
+          if (whole) {
+            *reinterpret_cast<uint4*>(at) = w;
+            continue;
+          }
+          const int left = a.n - (n + c + piece * kElems);
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < kElems; ++j) {
-        if (j < left) {
-          if constexpr (kSize == 4)
-            reinterpret_cast<uint32_t*>(at)[j] = words[j];
-          else
-            reinterpret_cast<uint16_t*>(at)[j] = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
+          for (int j = 0; j < kElems; ++j) {
+            if (j < left) {
+              if constexpr (kSize == 4)
+                reinterpret_cast<uint32_t*>(at)[j] = words[j];
+              else
+                reinterpret_cast<uint16_t*>(at)[j] = (uint16_t)(words[j / 2] >> (16 * (j & 1)));
+            }
+          }
+        }
+      } else {
+        // rows on no 16-byte boundaries: neighbouring lanes store neighbouring words (or 16-bit values) of a row.  Values
+        // one by one from the 16-byte pieces took 125 us for int8 30000 x 2000 x 700, whose products take 46.
+        const int log_each = args.align >= 4 ? 2 : 1, per_row = kStagingRow >> log_each;
+        const int at = lane % per_row << log_each;  // bytes into the staging row
+        const int left = a.n - (n + c) - at / kSize;
+        for (int first = 0; first < 32; first += 32 / per_row) {
+          const int row = first + lane / per_row, dst = __shfl_sync(0xffffffffu, r.dst, row);
+          if (dst < 0 || left <= 0) continue;
+          const uint32_t from = mine + place(row, at / 16) + at % 16;
+          uint8_t* out = static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + n + c) * kSize + at;
+          if (log_each == 2 && (kSize == 4 || left > 1)) {
+            uint32_t w;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from));
+            *reinterpret_cast<uint32_t*>(out) = w;
+          } else {
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(from));
+            *reinterpret_cast<uint16_t*>(out) = w;
+          }
         }
       }
-    }
     }
   }
 }
@@ -710,7 +733,7 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   // a unit of columns of 32 rows; tiles whose unit is narrower than a staging row store row by row
   constexpr int kSpan = S::kPart >= 64 ? S::kPart / 2 : S::kPart;
   const int size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
-  args.boxes = !SPLIT && args.wide && !a.out_rows && kSpan * size >= kStagingRow &&
+  args.boxes = !SPLIT && args.align == 16 && !a.out_rows && kSpan * size >= kStagingRow &&
                make_map(&map_out, 2, a.out_dtype, a.out, a.n, a.out_rows_total, a.out_ld, 1, 0, 32, kStagingRow);
   const auto kernel = eb_linear_kernel<I8, BN, CG, SPLIT>;
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel may use this much shared memory
@@ -754,19 +777,25 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   // The tile with the least estimated time: full waves of tiles (every group ends half a tile into its last one, on
   // average) at so many clocks per stage of K, plus the clocks that a tile costs beside its products, plus those of
   // storing the last one.  Wide tiles read x and the weights less often from L2, which bounds them; narrow ones give all
-  // SMs work.  Rows by index cannot be copied faster than 760 clocks per 128 of them and stage.  Clocks fitted to 29
-  // measured products (256 to 65536 rows, 256 to 15608 columns, 128 to 1024 units, 1 to 64 groups, int8 and bf16): the
-  // estimate's choice is within 2 % of the fastest tile for each of them, where no one tile is within 70 % for all.
+  // SMs work.  Rows by index cannot be copied faster than 850 clocks per 128 of them and stage.  Clocks fitted to 38
+  // measured products (256 to 65536 rows, 256 to 15608 columns, 128 to 1024 units, 1 to 64 groups, int8 and 16 bits): the
+  // estimate's choice is within 2 % of the fastest tile for each of them; each of the five is the fastest for some, and
+  // up to three times as slow as the fastest for others.
   struct Choice {
     int rows, cols, ctas, stage, tile, last;
   };
-  static const Choice choices[] = {{256, 512, 2, 1250, 7300, 4200}, {256, 256, 2, 630, 3100, 4700}, {128, 256, 1, 860, 3100, 1750},
-                                   {128, 128, 1, 410, 3100, 1200}, {128, 64, 1, 270, 3100, 0}};
+  static const Choice choices[] = {{256, 512, 2, 1370, 5100, 3280}, {256, 256, 2, 786, 1830, 3110}, {128, 256, 1, 883, 1830, 2190},
+                                   {128, 128, 1, 511, 1830, 550}, {128, 64, 1, 354, 1830, 0}};
   const int64_t groups = a.num_groups < a.positions ? a.num_groups : a.positions;
   auto clocks = [&](const Choice& c, int split) {
-    const int64_t tiles2 = (a.num_groups == 1 ? 2 * ((a.positions + c.rows - 1) / c.rows) : 2 * a.positions / c.rows + groups) * ((a.n + c.cols - 1) / c.cols);
+    int64_t tiles2 = 2 * ((a.positions + c.rows - 1) / c.rows);  // twice the tiles
+    if (a.num_groups > 1) {
+      tiles2 = 2 * a.positions / c.rows + groups;
+      if (tiles2 < 2 * groups) tiles2 = 2 * groups;
+    }
+    tiles2 *= (a.n + c.cols - 1) / c.cols;
     const int64_t slots2 = 2 * (sms / (c.ctas * split));
-    const int64_t stage = a.in_rows && c.stage < 760 ? 760 : c.stage;
+    const int64_t stage = a.in_rows && c.stage < 850 ? 850 : c.stage;
     const int64_t body = (args.k_steps + split - 1) / split * stage + c.tile;
     return (tiles2 + slots2 - 1) / slots2 * (body > c.last ? body : c.last) + c.last;
   };
@@ -774,12 +803,15 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   for (int i = 1; i < 5; ++i)
     if (clocks(choices[i], 1) < clocks(choices[best], 1)) best = i;
   int64_t least = clocks(choices[best], 1);
-  // K split over 2 or 4 CTAs, where they all run at once: joining the sums costs about 3700 clocks
+  // K split over 2 or 4 CTAs, where they all run at once: joining the sums costs about 6500 clocks
   int split = 1;
   for (int s = 2; s <= kMaxSplit; s *= 2) {
-    if (m128 * ((a.n + 63) / 64) * s > sms || s > args.k_steps) break;
-    if (clocks(choices[4], s) + 3700 < least) {
-      least = clocks(choices[4], s) + 3700;
+    // over 4 where even the most tiles that the groups can make run at once, over 2 where their likely number does
+    const int64_t likely = a.positions / 128 + groups / 2 > groups ? a.positions / 128 + groups / 2 : groups;
+    const int64_t tiles = s > 2 || a.num_groups == 1 ? m128 : likely;
+    if (tiles * ((a.n + 63) / 64) * s > sms / s * s || s > args.k_steps) break;
+    if (clocks(choices[4], s) + 6500 < least) {
+      least = clocks(choices[4], s) + 6500;
       split = s;
     }
   }
@@ -821,6 +853,10 @@ int eb_linear(const eb_linear_args* args, int device, void* stream) {
   if (a.positions == 0 || a.out_rows_total == 0) return EB_OK;
   if (!a.weight || !a.out || !a.status || (a.x_rows > 0 && !a.x) || (i8 && (!a.w_scale || (a.x_rows > 0 && !a.x_scale))))
     return linear_fail(EB_ERR_INVALID_ARG, "null pointer");
+  auto off = [](const void* p, int64_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+  if (off(a.bias, 4) || off(a.x_scale, 4) || off(a.w_scale, 4) || off(a.offsets, 4) || off(a.in_rows, 4) || off(a.out_rows, 4) ||
+      off(a.status, 4) || off(a.out, a.out_dtype == EB_OUT_F32 ? 4 : 2))
+    return linear_fail(EB_ERR_INVALID_ARG, "a pointer is not aligned to its elements");
   if (a.x_rows > 1 && a.x_ld < a.k) return linear_fail(EB_ERR_INVALID_ARG, "x_ld %lld below k", (long long)a.x_ld);
   if (a.w_ld < a.k || (a.num_groups > 1 && a.w_group_ld < a.w_ld * (a.n - 1) + a.k)) return linear_fail(EB_ERR_INVALID_ARG, "weight rows overlap");
   if (a.out_rows_total > 1 && a.out_ld < a.n) return linear_fail(EB_ERR_INVALID_ARG, "out_ld %lld below n", (long long)a.out_ld);
@@ -837,7 +873,7 @@ int eb_linear(const eb_linear_args* args, int device, void* stream) {
   LinearArgs la{};
   la.a = a;
   const int64_t size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
-  la.wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_ld * size % 16 == 0;
+  for (la.align = 16; la.align > size && (reinterpret_cast<uintptr_t>(a.out) % la.align || a.out_ld * size % la.align);) la.align = la.align == 16 ? 4 : 2;
   return i8 ? dispatch<true>(la, device, static_cast<cudaStream_t>(stream))
             : dispatch<false>(la, device, static_cast<cudaStream_t>(stream));
 }

@@ -159,7 +159,7 @@ def test_int8_linear_large(rows, k, n):
 
 # sizes that reach each of the tiles (512 and 256 columns on pairs of CTAs, 256, 128, 64 and 16 columns on one, K split
 # over two and four), with columns and K that end inside them
-TILES = [(16384, 15608, 1024), (16300, 15000, 1001), (9000, 6000, 1000), (4096, 1924, 333), (4096, 480, 1000),
+TILES = [(16384, 15608, 1024), (16300, 15000, 1001), (9000, 6000, 1000), (4096, 1924, 1000), (4096, 1924, 333), (4096, 480, 1000),
          (2000, 1924, 777), (1000, 1030, 65), (5000, 3001, 15), (512, 15608, 700), (333, 9001, 300)]
 
 

@@ -81,6 +81,9 @@ def product(lib, **kw):
     (dict(x_scale=None), _lib.EB_ERR_INVALID_ARG), (dict(w_scale=None), _lib.EB_ERR_INVALID_ARG),
     (dict(x_ld=16), _lib.EB_ERR_INVALID_ARG), (dict(w_ld=16), _lib.EB_ERR_INVALID_ARG),
     (dict(w_group_ld=496), _lib.EB_ERR_INVALID_ARG), (dict(out_ld=15), _lib.EB_ERR_INVALID_ARG),
+    (dict(out=P + 1), _lib.EB_ERR_INVALID_ARG), (dict(out=P + 2, out_dtype=_lib.EB_OUT_F32), _lib.EB_ERR_INVALID_ARG),
+    (dict(offsets=P + 2), _lib.EB_ERR_INVALID_ARG), (dict(in_rows=P + 1), _lib.EB_ERR_INVALID_ARG),
+    (dict(bias=P + 2), _lib.EB_ERR_INVALID_ARG), (dict(w_scale=P + 3), _lib.EB_ERR_INVALID_ARG),
     (dict(x=P + 8), _lib.EB_ERR_UNSUPPORTED), (dict(weight=P + 8), _lib.EB_ERR_UNSUPPORTED),
     (dict(x_ld=40), _lib.EB_ERR_UNSUPPORTED), (dict(w_ld=40, w_group_ld=1024), _lib.EB_ERR_UNSUPPORTED),
     (dict(w_group_ld=520), _lib.EB_ERR_UNSUPPORTED)])
