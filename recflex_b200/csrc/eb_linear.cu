@@ -12,12 +12,14 @@
 // whole row segments are stored, wherever their rows go.  Which tiles there are
 // follows from the offsets on the GPU; the host never reads them.
 //
-// What bounds it: the tensor units for long K (int8 16384 x 15608 x 1024 in
-// 0.169 ms, 3.1 Pop/s; bf16 of that size in 8 groups, rows by index, 0.395 ms,
-// 1.33 Pflop/s), and before them the way of the operands from L2 to the SMs,
-// about 55 bytes a clock and SM, which is why the widest tile wins there; for
-// short K the way from launch to the first products and from the last to the
-// stored results, about 8 us of int8 4096 x 1924 x 1024's 13.8.
+// What bounds it.  At long K the bandwidth of shared memory: products of
+// 256 x 256 x 32 bytes read 96 bytes a clock and SM, and the copies write 47
+// (512-column tiles) to 64 (256) beside them, of 128; the tensor pipes are 83 to
+// 88 % active (int8 16384 x 15608 x 1024 in 0.169 ms, 3.1 Pop/s; bf16 of that
+// size in 8 groups, rows by index, 0.395 ms, 1.33 Pflop/s).  At short K the
+// results' way out (65536 x 480 x 1024 in int8: 43 us, 3.9 TB/s), and in small
+// products the way from launch to the first copies and from the last product to
+// the stored results, about 8 us of int8 4096 x 1924 x 1024's 12.7.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -72,7 +72,9 @@ __device__ __forceinline__ const uint8_t* row_of(const eb_linear_args& a, int p,
 }
 
 // A CTA per run of units and tile of ROWS positions of one group; `share` of its warps split K, each set of warps takes 4
-// units.  Bound by the weights' bytes: each lane keeps 8 weight loads in flight, the rows of x come from L1 / L2.
+// units.  Bound by the weights' bytes: each lane keeps 8 weight loads in flight, the rows of x come from L1 / L2.  One
+// row of 15608 x 1024 takes 5.4 us in int8 (3.0 TB/s, launch included) and 8.0 in fp16 (4.0 TB/s); six rows over 16
+// experts of 1924 x 1024 in bf16 8.6.
 template <Kind KIND, int ROWS>
 __global__ void __launch_bounds__(kFewThreads) eb_linear_few_kernel(const __grid_constant__ eb_linear_args a, int share) {
   constexpr int kSize = KIND == kI8 ? 1 : 2, kPer = 16 / kSize;
@@ -144,7 +146,8 @@ __global__ void __launch_bounds__(kFewThreads) eb_linear_few_kernel(const __grid
 }
 
 // A layer of one unit over short rows: `lanes` lanes share a row of x (each 16 bytes of it at a time), every set of lanes
-// keeps 4 rows in flight.  Bound by the bytes of x; the weights come from L1.
+// keeps 4 rows in flight.  Bound by the bytes of x; the weights come from L1.  65536 int8 rows of 128 take 4.6 us
+// (1.9 TB/s, launch included).
 template <Kind KIND>
 __global__ void __launch_bounds__(kFewThreads) eb_linear_narrow_kernel(const __grid_constant__ eb_linear_args a, int lanes) {
   constexpr int kSize = KIND == kI8 ? 1 : 2, kPer = 16 / kSize, kRows = 4;
