@@ -54,27 +54,37 @@ def check_status(device=None) -> None:
         _lib.check(_lib.load().eb_linear_check_status(word[1], index, torch.cuda.current_stream(index).cuda_stream))
 
 
-def _check(name: str, t: torch.Tensor, dims: int, dtypes, device: Optional[torch.device] = None) -> None:
-    if type(t) is torch.Tensor and t.is_cuda and t.dim() == dims and t.dtype in dtypes and not t.requires_grad \
-            and (device is None or t.get_device() == device.index):
-        return
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+_Tensor = torch.Tensor
+_I8, _I32 = (torch.int8,), (torch.int32,)
+# the current stream's handle by device index, without the stream object around it
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _check(name: str, t: torch.Tensor, dims: int, dtypes, index: Optional[int] = None) -> int:
+    """The index of the device of a tensor argument that is what it has to be.  (What a call checks first is what costs
+    least to ask for; the rest words the refusal.)"""
+    if type(t) is _Tensor and t.dtype in dtypes and t.dim() == dims and not t.requires_grad:
+        at = t.get_device()
+        if at == index or (index is None and at >= 0 and t.is_cuda):
+            return at
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must live on {device}, it lives on {t.device}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} must live on cuda:{index}, it lives on {t.device}")
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, it has {t.dim()}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these layers are forward only (detach it or use torch.no_grad())")
+    return t.get_device()
 
 
-def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == device.index and t.shape == shape \
-            and t.is_contiguous() and not t.requires_grad:
+def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, index: int) -> torch.Tensor:
+    if type(t) is _Tensor and t.dtype is dtype and t.is_contiguous() and t.get_device() == index and not t.requires_grad \
+            and (t.numel() == shape[0] and t.dim() == 1 if len(shape) == 1 else t.shape == shape):
         return t
-    _check(name, t, len(shape), (dtype,), device)
+    _check(name, t, len(shape), (dtype,), index)
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)}, it is {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
@@ -123,10 +133,6 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + last * t.element_size()
 
 
-# the current stream's handle by device index, without the stream object around it
-_current_stream = torch._C._cuda_getCurrentRawStream
-
-
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows in 8 bits with one scale a row: `(q, scale)` with `q` int8 `[rows, k]`, `scale` float32 `[rows]`.
 
@@ -134,16 +140,17 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     scale 0; a row that holds an infinity or a NaN has codes 0 and a scale that is not finite, so that its products are
     NaN.  `x`: `[rows, k]` float32, bfloat16 or float16 with any strides.  The rows of `q` start on 16-byte boundaries.
     """
-    _check("x", x, 2, _FLOATS)
+    index = _check("x", x, 2, _FLOATS)
     rows, k = x.shape
-    if k > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < k:
+    ld, step = x.stride()
+    if k > 1 and step != 1 or rows > 1 and ld < k:
         x = x.contiguous()
+        ld = k
     device, q_ld = x.device, (k + 15) // 16 * 16
     q = torch.empty_strided((rows, k), (q_ld, 1), dtype=torch.int8, device=device)
     scale = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device)
-    code = _lib.load().eb_quantize_rows(x.data_ptr(), rows, k, x.stride(0) if rows > 1 else k, _FLOATS[x.dtype],
-                                        q.data_ptr(), q_ld, scale.data_ptr(), device.index,
-                                        _current_stream(device.index))
+    code = _lib.load().eb_quantize_rows(x.data_ptr(), rows, k, ld if rows > 1 else k, _FLOATS[x.dtype], q.data_ptr(), q_ld,
+                                        scale.data_ptr(), index, _current_stream(index))
     if code:
         _lib.check(code)
     return q, scale
@@ -156,7 +163,7 @@ def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, tor
     rows in increasing order, then the rows whose number lies outside `[0, num_groups)` (-1 for padding, say).  Expert
     g owns `order[offsets[g]:offsets[g + 1]]`: the `offsets` that `grouped_linear` takes.
     """
-    _check("groups", groups, 1, _INDEX)
+    index = _check("groups", groups, 1, _INDEX)
     if not groups.is_contiguous():
         groups = groups.contiguous()
     rows, device, lib, num_groups = groups.shape[0], groups.device, _lib.load(), int(num_groups)
@@ -167,15 +174,14 @@ def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, tor
     if not code:
         ws = torch.empty_strided((need.value,), (1,), dtype=torch.uint8, device=device) if need.value else None
         code = lib.eb_group_rows(groups.data_ptr(), rows, num_groups, _INDEX[groups.dtype], order.data_ptr(),
-                                 offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, device.index,
-                                 _current_stream(device.index))
+                                 offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, index,
+                                 _current_stream(index))
     if code:
         _lib.check(code)
     return order, offsets
 
 
-def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out):
-    device = x.device
+def _product(index, x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out):
     x_rows, k = x.shape
     if weight.dim() == 3:
         groups, n, w_k = weight.shape
@@ -194,26 +200,26 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
     positions = x_rows
     in_ptr = out_ptr = offsets_ptr = bias_ptr = x_scale_ptr = w_scale_ptr = 0
     if in_rows is not None:
-        _check("in_rows", in_rows, 1, (torch.int32,), device)
-        in_rows = in_rows.contiguous()
+        _check("in_rows", in_rows, 1, _I32, index)
+        in_rows = in_rows if in_rows.is_contiguous() else in_rows.contiguous()
         positions, in_ptr = in_rows.shape[0], in_rows.data_ptr()
     if out_rows is not None:
-        _check("out_rows", out_rows, 1, (torch.int32,), device)
+        _check("out_rows", out_rows, 1, _I32, index)
         if out_rows.shape[0] != positions:
             raise ValueError(f"out_rows has {out_rows.shape[0]} entries for {positions} rows")
-        out_rows = out_rows.contiguous()
+        out_rows = out_rows if out_rows.is_contiguous() else out_rows.contiguous()
         out_ptr = out_rows.data_ptr()
     if offsets is not None:
-        offsets = _vector("offsets", offsets, (groups + 1,), torch.int32, device)
+        offsets = _vector("offsets", offsets, (groups + 1,), torch.int32, index)
         offsets_ptr = offsets.data_ptr()
     if bias is not None:
-        bias = _vector("bias", bias, lead, torch.float32, device)
+        bias = _vector("bias", bias, lead, torch.float32, index)
         bias_ptr = bias.data_ptr()
     if x.dtype is torch.int8:
         if x_scale is None or weight_scale is None:
             raise ValueError("8-bit products need x_scale and weight_scale")
-        x_scale = _vector("x_scale", x_scale, (x_rows,), torch.float32, device)
-        weight_scale = _vector("weight_scale", weight_scale, lead, torch.float32, device)
+        x_scale = _vector("x_scale", x_scale, (x_rows,), torch.float32, index)
+        weight_scale = _vector("weight_scale", weight_scale, lead, torch.float32, index)
         x_scale_ptr, w_scale_ptr = x_scale.data_ptr(), weight_scale.data_ptr()
         dtype = _lib.EB_ROW_I8
         if out_dtype is None:
@@ -232,13 +238,13 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
     if out is None:
         # without out_rows every position is a row of the result, and the kernel fills those of no group with zeros
         if out_rows is None:
-            out = torch.empty_strided((positions, n), (n, 1), dtype=out_dtype, device=device)
+            out = torch.empty_strided((positions, n), (n, 1), dtype=out_dtype, device=x.device)
             zero_rest = int(offsets is not None)
         else:
-            out = torch.zeros((positions, n), dtype=out_dtype, device=device)
+            out = torch.zeros((positions, n), dtype=out_dtype, device=x.device)
         result_rows, out_ld = positions, n
     else:
-        _check("out", out, 2, (out_dtype,), device)
+        _check("out", out, 2, (out_dtype,), index)
         if out.shape[1] != n or (n > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < n):
             raise ValueError(f"out must be [rows, {n}] with unit column stride and rows that do not overlap")
         if out_rows is None and out.shape[0] < positions:
@@ -251,18 +257,27 @@ def _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_row
                     raise ValueError("out must not share memory with the arguments")
         result_rows = out.shape[0]
         out_ld = out.stride(0) if result_rows > 1 else n
-    x_strides, w_strides = _wide_strides(x), _wide_strides(weight)
-    if x_strides is None:
-        x = pack_rows(x)
-        x_strides = _wide_strides(x)
-    if w_strides is None:
-        weight = pack_rows(weight)
-        w_strides = _wide_strides(weight)
-    index = device.index
-    args = _lib.pack_linear_args(x.data_ptr(), weight.data_ptr(), bias_ptr, x_scale_ptr, w_scale_ptr, offsets_ptr, in_ptr,
-                                 out_ptr, out.data_ptr(), _status_word(index), x_rows, x_strides[0], w_strides[0],
-                                 w_strides[1], positions, result_rows, out_ld, n, k, groups, dtype, out_code, act,
-                                 zero_rest)
+    # layouts that are read in place; the usual ones are recognised without asking for everything (_wide_strides)
+    x_ptr, weight_ptr, (x_ld, step) = x.data_ptr(), weight.data_ptr(), x.stride()
+    per = 16 if dtype == _lib.EB_ROW_I8 else 8
+    if step != 1 or x_ld % per or x_ld < k or x_ptr % 16:
+        strides = _wide_strides(x)
+        if strides is None:
+            x = pack_rows(x)
+            strides = _wide_strides(x)
+        x_ld, x_ptr = strides[0], x.data_ptr()
+    w_strides = weight.stride()
+    if groups == 1 and w_strides[-1] == 1 and w_strides[-2] % per == 0 and w_strides[-2] >= k and weight_ptr % 16 == 0:
+        w_ld, w_group_ld = w_strides[-2], w_strides[-2] * n
+    else:
+        strides = _wide_strides(weight)
+        if strides is None:
+            weight = pack_rows(weight)
+            strides = _wide_strides(weight)
+        (w_ld, w_group_ld), weight_ptr = strides, weight.data_ptr()
+    args = _lib.pack_linear_args(x_ptr, weight_ptr, bias_ptr, x_scale_ptr, w_scale_ptr, offsets_ptr, in_ptr, out_ptr,
+                                 out.data_ptr(), _status_word(index), x_rows, x_ld, w_ld, w_group_ld, positions,
+                                 result_rows, out_ld, n, k, groups, dtype, out_code, act, zero_rest)
     code = _lib.load().eb_linear(args, index, _current_stream(index))
     if code:
         _lib.check(code)
@@ -278,9 +293,9 @@ def int8_linear(q: torch.Tensor, q_scale: torch.Tensor, weight: torch.Tensor, we
     `weight_scale` float32 `[n]`; `bias` float32 `[n]`.  The products are summed exactly in 32-bit integers (k up to
     131071), scaled in fp32 and rounded once to `out_dtype` (float32, bfloat16, the default, or float16).
     """
-    _check("q", q, 2, (torch.int8,))
-    _check("weight", weight, 2, (torch.int8,), q.device)
-    return _product(q, weight, bias, activation, q_scale, weight_scale, None, None, None, out_dtype, out)
+    index = _check("q", q, 2, _I8)
+    _check("weight", weight, 2, _I8, index)
+    return _product(index, q, weight, bias, activation, q_scale, weight_scale, None, None, None, out_dtype, out)
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -299,11 +314,11 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     Positions of no expert (behind the last offset, or in front of the first) give rows of zeros when the result is
     allocated here, and leave the rows of a given `out` as they were.  No row number may stand twice in `out_rows`.
     """
-    _check("x", x, 2, (torch.bfloat16, torch.float16, torch.int8))
-    _check("weight", weight, 3, (x.dtype,), x.device)
+    index = _check("x", x, 2, (torch.bfloat16, torch.float16, torch.int8))
+    _check("weight", weight, 3, (x.dtype,), index)
     if offsets is None:
         raise ValueError("offsets must be an int32 tensor")
-    return _product(x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out)
+    return _product(index, x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out)
 
 
 class Int8Linear(nn.Module):

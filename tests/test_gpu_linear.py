@@ -596,6 +596,43 @@ def test_captured_and_replayed_beside_eager_calls_on_another_stream(quantized):
     linear.check_status(DEV)
 
 
+def test_two_threads_on_two_streams():
+    """Calls of every kind at once: nothing but the status word is shared between them."""
+    import threading
+
+    g = gen(23)
+    layers = [chain_layers(g, False), chain_layers(g, True)]
+    x = torch.randn(3000, 200, generator=g, device=DEV).bfloat16()
+    ids = torch.randint(-1, 5, (3000,), generator=g, device=DEV)
+    big_q, big_w = codes((2048, 4000), g), codes((1024, 4000), g)
+    qs, ws = scales(2048, g), scales(1024, g)
+
+    def once(i):
+        return (chain(x, ids, *layers[i]), linear.int8_linear(big_q, qs, big_w, ws, None, "relu"),
+                linear.int8_linear(big_q[:1], qs[:1], big_w, ws), linear.int8_linear(big_q[:200], qs[:200], big_w[:64], ws[:64]))
+
+    want = [once(0), once(1)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(40):
+                    got = once(i)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        failed.append(i)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed
+    linear.check_status(DEV)
+
+
 def pooled_model(**kw):
     from .helpers import device_tables, small_model, to_device
     from recflex_b200.rec_modules import RecomModel
