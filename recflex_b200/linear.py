@@ -11,6 +11,7 @@ fault, and `check_status` reports them.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import threading
 from typing import Optional, Tuple
 
@@ -156,6 +157,14 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
+@functools.lru_cache(maxsize=256)
+def _group_workspace(rows: int, num_groups: int) -> int:
+    """Bytes of scratch that eb_group_rows needs for these sizes."""
+    need = C.c_size_t()
+    _lib.check(_lib.load().eb_group_rows_workspace_bytes(rows, num_groups, C.byref(need)))
+    return need.value
+
+
 def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows by expert: `(order, offsets)`, both int32.
 
@@ -166,16 +175,14 @@ def group_rows(groups: torch.Tensor, num_groups: int) -> Tuple[torch.Tensor, tor
     index = _check("groups", groups, 1, _INDEX)
     if not groups.is_contiguous():
         groups = groups.contiguous()
-    rows, device, lib, num_groups = groups.shape[0], groups.device, _lib.load(), int(num_groups)
+    rows, device, num_groups = groups.shape[0], groups.device, int(num_groups)
+    need = _group_workspace(rows, num_groups)
     order = torch.empty_strided((rows,), (1,), dtype=torch.int32, device=device)
-    offsets = torch.empty_strided((max(0, num_groups) + 1,), (1,), dtype=torch.int32, device=device)
-    need = C.c_size_t()
-    code = lib.eb_group_rows_workspace_bytes(rows, num_groups, C.byref(need))
-    if not code:
-        ws = torch.empty_strided((need.value,), (1,), dtype=torch.uint8, device=device) if need.value else None
-        code = lib.eb_group_rows(groups.data_ptr(), rows, num_groups, _INDEX[groups.dtype], order.data_ptr(),
-                                 offsets.data_ptr(), ws.data_ptr() if need.value else None, need.value, index,
-                                 _current_stream(index))
+    offsets = torch.empty_strided((num_groups + 1,), (1,), dtype=torch.int32, device=device)
+    ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None
+    code = _lib.load().eb_group_rows(groups.data_ptr(), rows, num_groups, _INDEX[groups.dtype], order.data_ptr(),
+                                     offsets.data_ptr(), ws.data_ptr() if need else None, need, index,
+                                     _current_stream(index))
     if code:
         _lib.check(code)
     return order, offsets

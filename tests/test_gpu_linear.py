@@ -596,6 +596,41 @@ def test_captured_and_replayed_beside_eager_calls_on_another_stream(quantized):
     linear.check_status(DEV)
 
 
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 9, 40])
+def test_chain_of_few_rows(rows, quantized):
+    """Group, first layer by index, last layer back in order, for one request to a handful: against float64."""
+    g = gen(50 + rows)
+    first, second = chain_layers(g, quantized)
+    x = torch.randn(rows, 200, generator=g, device=DEV).bfloat16()
+    ids = torch.randint(-1, 5, (rows,), generator=g, device=DEV)
+    got = chain(x, ids, first, second)
+    assert got.shape == (rows, 1)
+
+    def layer(rows_in, l, e):  # the rows and weights that the layer multiplies, in 64 bits
+        if not quantized:
+            return rows_in.double() @ l.weight[e].double().t()
+        q, s = linear.quantize_rows(rows_in)
+        return int_product(q, l.weight[e]) * s.double()[:, None] * l.weight_scale[e].double()
+
+    for r in range(rows):
+        e = int(ids[r])
+        if e < 0:
+            assert got[r] == 0
+            continue
+        h = torch.relu(layer(x[r:r + 1], first, e) + first.bias[e].double())
+        y = torch.sigmoid(layer(h.bfloat16(), second, e))
+        # every hidden value may have fallen to the other side of a border of bf16: one step, at most eps of it.  In 8 bits
+        # each is then off by half a unit of the scale on either side, the scale itself by one step of the largest.  All of
+        # it goes through the second layer's weights, the sigmoid's slope (1/4 at most) and the result's own rounding
+        # (half a step of at most 1); 2^-20 covers the fp32 sums and the sigmoid.
+        w = second.weight[e].double().abs() * (second.weight_scale[e].double()[:, None] if quantized else 1)
+        off = h.abs() * 2.0 ** -7 + (h.abs().max() / 127 * (1 + 2.0 ** -7) if quantized else 0)
+        slack = (off @ w.t()).item() / 4 + half_step(torch.bfloat16) + 2.0 ** -20
+        assert (got[r].double() - y[0]).abs() <= slack
+    linear.check_status(DEV)
+
+
 def test_two_threads_on_two_streams():
     """Calls of every kind at once: nothing but the status word is shared between them."""
     import threading
