@@ -221,6 +221,29 @@ def test_int8_linear_layouts_and_given_out():
         assert (wide[:, :11] == 7).all() and (wide[:, 61:] == 7).all() and (wide[q.shape[0]:] == 7).all()
 
 
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 20, 33, 36, 129, 250, 252, 500])
+@pytest.mark.parametrize("kind", ["i8", "bf16"])
+def test_results_rows_are_on_wide_boundaries_or_packed_as_given(kind, n):
+    g = gen(n)
+    for rows, out_dtype in ((3, None), (700, None)) + (((700, torch.float32),) if kind == "i8" else ()):
+        x, w, kw = codes((rows, 40), g), codes((2, n, 40), g), dict(x_scale=scales(rows, g), weight_scale=scales(2 * n, g).view(2, n))
+        if kind == "bf16":
+            x, w, kw = x.bfloat16(), w.bfloat16(), {}
+        order, offsets = linear.group_rows(torch.randint(0, 2, (rows,), generator=g, device=DEV), 2)
+        for out_rows in (None, order):
+            got = linear.grouped_linear(x, w, offsets, out_rows=out_rows, out_dtype=out_dtype, **kw)
+            per = 16 // got.dtype.itemsize
+            assert got.stride() == (n if n <= 16 else -(-n // per) * per, 1)
+            packed = torch.full((rows, n), 7.0, dtype=got.dtype, device=DEV)
+            linear.grouped_linear(x, w, offsets, out_rows=out_rows, out_dtype=out_dtype, out=packed, **kw)
+            assert torch.equal(packed, got)
+            exact, slack = plain_grouped(x, w, offsets, None, "none", None, out_rows, torch.zeros_like(got), kw.get("x_scale"), kw.get("weight_scale"))
+            check(got, exact, slack)
+        if n > 16 and out_dtype is None:
+            # the next product reads such rows where they lie
+            assert linear.pack_rows(got) is got
+
+
 def test_rows_that_are_not_finite_give_nan_and_leave_the_others_alone():
     g = gen(4)
     x = torch.randn(40, 100, generator=g, device=DEV)
