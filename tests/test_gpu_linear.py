@@ -221,6 +221,24 @@ def test_int8_linear_layouts_and_given_out():
         assert (wide[:, :11] == 7).all() and (wide[:, 61:] == 7).all() and (wide[q.shape[0]:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows, n", [(2, 512), (40, 1), (300, 16), (900, 512), (900, 100)])
+def test_sigmoid_over_its_range(rows, n, dtype):
+    """Rows of zeros give sigmoid(bias) exactly as the kernel evaluates it: relative to the value, up to where it is 0."""
+    bias = torch.linspace(-87, 87, n, device=DEV) if n > 1 else torch.full((1,), -40.0, device=DEV)
+    if n > 4:
+        bias[:4] = torch.tensor([0.0, float("inf"), -float("inf"), -1e4], device=DEV)
+    zero = torch.zeros(max(rows, n), 64, dtype=torch.int8, device=DEV)
+    scale = torch.ones(max(rows, n), device=DEV)
+    out = linear.int8_linear(zero[:rows], scale[:rows], zero[:n], scale[:n], bias, "sigmoid", dtype)
+    want = torch.sigmoid(bias.double()).expand(rows, n)
+    # expf 2 units of 2^-23, the sum half a unit, the quotient 2 units; then the rounding to `dtype`, and where that type
+    # ends half its smallest step (fp32: values below 2^-126 may be 0)
+    tiny = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[dtype]
+    assert ((out.double() - want).abs() <= want * (4.5 * 2.0 ** -23 + half_step(dtype)) * (1 + 2.0 ** -10) + tiny).all()
+    assert torch.isnan(linear.int8_linear(zero[:rows], scale[:rows], zero[:n], scale[:n], bias * float("nan"), "sigmoid", dtype)).all()
+
+
 @pytest.mark.parametrize("n", [1, 15, 16, 17, 20, 33, 36, 129, 250, 252, 500])
 @pytest.mark.parametrize("kind", ["i8", "bf16"])
 def test_results_rows_are_on_wide_boundaries_or_packed_as_given(kind, n):
