@@ -779,16 +779,18 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   // The tile with the least estimated time: full waves of tiles (every group ends half a tile into its last one, on
   // average) at so many clocks per stage of K, plus the clocks that a tile costs beside its products, plus those of
   // storing the last one.  Wide tiles read x and the weights less often from L2, which bounds them; narrow ones give all
-  // SMs work.  Rows by index cannot be copied faster than 850 clocks per 128 of them and stage.  Clocks fitted to 38
+  // SMs work.  Rows by index cannot be copied faster than 350 to 850 clocks a stage for few to 128.  Clocks fitted to 38
   // measured products (256 to 65536 rows, 256 to 15608 columns, 128 to 1024 units, 1 to 64 groups, int8 and 16 bits): the
   // estimate's choice is within 2 % of the fastest tile for each of them; each of the five is the fastest for some, and
   // up to three times as slow as the fastest for others.
   struct Choice {
     int rows, cols, ctas, stage, tile, last;
   };
-  static const Choice choices[] = {{256, 512, 2, 1370, 5100, 3280}, {256, 256, 2, 786, 1830, 3110}, {128, 256, 1, 883, 1830, 2190},
+  static const Choice choices[] = {{256, 512, 2, 1370, 5800, 3280}, {256, 256, 2, 786, 1830, 3110}, {128, 256, 1, 883, 1830, 2190},
                                    {128, 128, 1, 511, 1830, 550}, {128, 64, 1, 354, 1830, 0}};
   const int64_t groups = a.num_groups < a.positions ? a.num_groups : a.positions;
+  const int64_t each = a.positions / groups < 128 ? a.positions / groups : 128;  // rows of a tile
+  const int64_t least_stage = a.in_rows ? 350 + 4 * each : 0;
   auto clocks = [&](const Choice& c, int split) {
     int64_t tiles2 = 2 * ((a.positions + c.rows - 1) / c.rows);  // twice the tiles
     if (a.num_groups > 1) {
@@ -797,7 +799,7 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
     }
     tiles2 *= (a.n + c.cols - 1) / c.cols;
     const int64_t slots2 = 2 * (sms / (c.ctas * split));
-    const int64_t stage = a.in_rows && c.stage < 850 ? 850 : c.stage;
+    const int64_t stage = c.stage < least_stage ? least_stage : c.stage;
     const int64_t body = (args.k_steps + split - 1) / split * stage + c.tile;
     return (tiles2 + slots2 - 1) / slots2 * (body > c.last ? body : c.last) + c.last;
   };
@@ -805,15 +807,18 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   for (int i = 1; i < 5; ++i)
     if (clocks(choices[i], 1) < clocks(choices[best], 1)) best = i;
   int64_t least = clocks(choices[best], 1);
-  // K split over 2 or 4 CTAs, where they all run at once: joining the sums costs about 6500 clocks
+  // K split over 2 or 4 CTAs, where they all run at once (clusters of 4 leave some SMs out: 31 of them ran at once, 33 did
+  // not).  Joining the sums costs 5000 clocks for a few rows and 12000 for 128, measured at 80 products: int8
+  // 938 x 3828 x 101 takes 10.3 us whole, over 4 CTAs 12.5; 918 x 24160 x 256 39.3 and 21.0.
+  const int64_t join = 5500 + 50 * each;
   int split = 1;
   for (int s = 2; s <= kMaxSplit; s *= 2) {
     // over 4 where even the most tiles that the groups can make run at once, over 2 where their likely number does
     const int64_t likely = a.positions / 128 + groups / 2 > groups ? a.positions / 128 + groups / 2 : groups;
     const int64_t tiles = s > 2 || a.num_groups == 1 ? m128 : likely;
-    if (tiles * ((a.n + 63) / 64) * s > sms / s * s || s > args.k_steps) break;
-    if (clocks(choices[4], s) + 6500 < least) {
-      least = clocks(choices[4], s) + 6500;
+    if (tiles * ((a.n + 63) / 64) * s > (s > 2 ? sms * 7 / 8 : sms) / s * s || s > args.k_steps) break;
+    if (clocks(choices[4], s) + join < least) {
+      least = clocks(choices[4], s) + join;
       split = s;
     }
   }
