@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "../../include/recflex_b200.h"
@@ -832,6 +833,15 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   }
 }
 
+// The status word as the last check found it: all streams set bits in a word, so reading and clearing it is one operation
+// (copied and then cleared, 198 of 2000 reports of another stream were lost between the two).
+__device__ uint32_t g_found;
+
+__global__ void take_status_kernel(uint32_t* status) { g_found = atomicExch(status, 0u); }
+
+// One check at a time uses a device's g_found; a check lasts until its stream has been waited for.
+std::mutex g_found_lock[kMaxDevices];
+
 }  // namespace
 }  // namespace ebk
 
@@ -887,12 +897,16 @@ int eb_linear(const eb_linear_args* args, int device, void* stream) {
 
 int eb_linear_check_status(uint32_t* status, int device, void* stream) {
   if (!status) return linear_fail(EB_ERR_INVALID_ARG, "null argument");
+  if (reinterpret_cast<uintptr_t>(status) % 4) return linear_fail(EB_ERR_INVALID_ARG, "the status word is not aligned");
+  if (device < 0 || device >= kMaxDevices) return linear_fail(EB_ERR_INVALID_ARG, "device %d out of range", device);
   DeviceScope scope(device);
   if (!scope.ok) return linear_fail(EB_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> lock(g_found_lock[device]);
   uint32_t host = 0;
-  cudaError_t e = cudaMemcpyAsync(&host, status, sizeof(host), cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaMemsetAsync(status, 0, sizeof(uint32_t), st);
+  take_status_kernel<<<1, 1, 0, st>>>(status);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&host, g_found, sizeof(host), 0, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return linear_fail(EB_ERR_CUDA, "eb_linear_check_status: %s", cudaGetErrorString(e));
   if (host & kLinearGaveUp) return linear_fail(EB_ERR_CUDA, "a kernel gave up waiting for its own copies; its results are not valid");

@@ -45,7 +45,10 @@ def _status_word(index: int) -> int:
 
 
 def check_status(device=None) -> None:
-    """Raise if a product since the last check met offsets or row numbers outside their range (synchronises)."""
+    """Raise if a product since the last check met offsets or row numbers outside their range.
+
+    Waits for the device's current stream and answers for the products in front of it there; what products on other
+    streams report is seen by this check or by the next one, whichever comes after it."""
     device = torch.device("cuda" if device is None else device)
     if device.type != "cuda":
         raise ValueError(f"check_status needs a CUDA device, got {device}")
