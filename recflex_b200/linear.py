@@ -5,8 +5,8 @@ these.  All of them call librecflex_b200.so (`eb_quantize_rows`, `eb_linear`, `e
 never synchronise with the host, and may be captured into a CUDA graph once one of them has run on the device.
 
 They are forward only, like the embedding layer in front of them: an argument that requires a gradient is refused
-while gradients are being recorded.  Row numbers and offsets live on the GPU and are checked there: bad ones never
-fault, and `check_status` reports them.
+while gradients are being recorded, and so is one that carries a forward-mode tangent.  Row numbers and offsets live
+on the GPU and are checked there: bad ones never fault, and `check_status` reports them.
 """
 from __future__ import annotations
 
@@ -16,6 +16,7 @@ import threading
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 import torch.nn as nn
 
 from . import _lib
@@ -67,7 +68,7 @@ _current_stream = torch._C._cuda_getCurrentRawStream
 def _check(name: str, t: torch.Tensor, dims: int, dtypes, index: Optional[int] = None) -> int:
     """The index of the device of a tensor argument that is what it has to be.  (What a call checks first is what costs
     least to ask for; the rest words the refusal.)"""
-    if type(t) is _Tensor and t.dtype in dtypes and t.dim() == dims and not t.requires_grad:
+    if type(t) is _Tensor and t.dtype in dtypes and t.dim() == dims and not t.requires_grad and _forward_ad._current_level < 0:
         at = t.get_device()
         if at == index or (index is None and at >= 0 and t.is_cuda):
             return at
@@ -81,12 +82,14 @@ def _check(name: str, t: torch.Tensor, dims: int, dtypes, index: Optional[int] =
         raise TypeError(f"{name}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these layers are forward only (detach it or use torch.no_grad())")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent: these layers are forward only (take its primal)")
     return t.get_device()
 
 
 def _vector(name: str, t: torch.Tensor, shape, dtype: torch.dtype, index: int) -> torch.Tensor:
     if type(t) is _Tensor and t.dtype is dtype and t.is_contiguous() and t.get_device() == index and not t.requires_grad \
-            and (t.numel() == shape[0] and t.dim() == 1 if len(shape) == 1 else t.shape == shape):
+            and _forward_ad._current_level < 0 and (t.numel() == shape[0] and t.dim() == 1 if len(shape) == 1 else t.shape == shape):
         return t
     _check(name, t, len(shape), (dtype,), index)
     if tuple(t.shape) != tuple(shape):

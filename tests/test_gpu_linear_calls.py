@@ -1,6 +1,7 @@
 """GPU: the dense layers around the products: reports, gradients, modules that move, the sigmoid's ends, long rows."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from recflex_b200 import _lib, linear
 
@@ -43,3 +44,34 @@ def test_no_report_is_lost_to_a_check_on_another_stream():
         side.synchronize()
         lost += not (reported() or first)
     assert lost == 0
+
+
+def test_forward_mode_tangents_are_refused():
+    """These layers have no derivative: a dual tensor's tangent would be dropped."""
+    x = torch.randn(8, 32, device=DEV)
+    h = x.bfloat16()
+    w = torch.randn(2, 16, 32, device=DEV).bfloat16()
+    off = torch.tensor([0, 4, 8], dtype=torch.int32, device=DEV)
+    bias = torch.zeros(2, 16, device=DEV)
+    q, qs = linear.quantize_rows(x)
+    wq, ws = linear.quantize_rows(w[0])
+    layer = linear.Int8Linear(w[0].float())
+    experts = linear.GroupedLinear(w)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: linear.quantize_rows(dual(x)), lambda: linear.quantize_rows(dual(x)[:, 1:]),
+                 lambda: linear.int8_linear(q, dual(qs), wq, ws), lambda: linear.int8_linear(q, qs, wq, dual(ws)),
+                 lambda: linear.int8_linear(q, qs, wq, ws, dual(bias[0])),
+                 lambda: linear.grouped_linear(dual(h), w, off), lambda: linear.grouped_linear(h, dual(w), off),
+                 lambda: linear.grouped_linear(h, w, off, dual(bias)), lambda: linear.grouped_linear(h, w, off, out=dual(h[:, :16].clone())),
+                 lambda: layer(dual(x)), lambda: experts(dual(h), off)]
+        for i, call in enumerate(calls):
+            with pytest.raises(ValueError, match="forward only"):
+                call()
+                pytest.fail(f"call {i} dropped a tangent")
+        want = linear.grouped_linear(h, w, off)  # arguments without one are taken
+        with torch.inference_mode():  # nothing is recorded
+            assert torch.equal(linear.grouped_linear(h, w, off), want)
+    assert torch.equal(linear.grouped_linear(h, w, off), want)
