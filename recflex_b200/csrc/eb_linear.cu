@@ -260,8 +260,9 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
 // SPLIT (CG = 1): the CTAs of a cluster share a tile and take a piece of K each; their accumulators are added through
 // distributed shared memory in the order of their ranks, so that the result is the same on every run.  All warps meet
 // at two cluster barriers a tile, also when one gave up.
-// Every wait ends: after two seconds a thread gives up, sets a bit of the status word, and the CTA drains what is under
-// way and returns.
+// Every wait ends: after two seconds in which nothing moved a thread gives up, sets a bit of the status word, and the CTA
+// drains what is under way and returns.  The wait for a tile's sums lasts for all of its stages (k = 2^30: 16.8 M of
+// them, 4.7 seconds), so it watches the copies: they go on until the last ten stages, or stop with what they wait for.
 template <bool I8, int BN, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     eb_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ CUtensorMap map_x,
@@ -282,9 +283,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t full = bars, empty = bars + 8 * kStages, done = bars + 16 * kStages, drained = done + 16, last = drained + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(after + 16 * kStages + 40);
   volatile int* gave_up = reinterpret_cast<volatile int*>(after + 16 * kStages + 44);
+  volatile uint32_t* moved = reinterpret_cast<volatile uint32_t*>(after + 16 * kStages + 48);  // stages filled so far
   int* off = reinterpret_cast<int*>(after + 256);
   int* tiles = off + a.num_groups + 1;
-  static_assert(16 * kStages + 48 <= 256, "barriers");
+  static_assert(16 * kStages + 52 <= 256, "barriers");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = CG > 1 || SPLIT ? cluster_rank() : 0;
@@ -310,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       bar_init(last, 1);
       *gave_up = 0;
+      *moved = 0;
       bar_init_done();
     }
     __syncwarp();
@@ -402,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_2d<CG>(sx + warp * kBoxRows * kKBytes, &map_x, k * kStep, m_cta + warp * kBoxRows, bar);
           }
           ++copied;
+          if (warp == 0) *moved = copied;
           if (++st == kStages) {
             st = 0;
             phase ^= 1;
@@ -559,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
-          ok = __all_sync(0xffffffffu, bar_wait(done + 8 * slot, turn & 1, gave_up));
+          ok = __all_sync(0xffffffffu, bar_wait(done + 8 * slot, turn & 1, gave_up, moved));
           if (!ok) break;
           fence_after();
           // on their way while this part is stored
@@ -602,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // every CTA lays its partial sums out in its ring (all its copies and products are done)
         constexpr int kPieces = BN / 4;  // of 16 bytes in a row
         const uint32_t acc = count & 1, d = tmem + acc * BN + ((uint32_t)(quad * 32) << 16);
-        ok = ok && __all_sync(0xffffffffu, bar_wait(done + 8 * acc, (count >> 1) & 1, gave_up));
+        ok = ok && __all_sync(0xffffffffu, bar_wait(done + 8 * acc, (count >> 1) & 1, gave_up, moved));
         fence_after();
         if (ok && quad * 32 < rows) {
           for (int c = half * 32; c < BN; c += 64) {

@@ -71,16 +71,23 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 }
 constexpr long long kWaitLimitClocks = 4000000000ll;  // two seconds at the highest clock
 
-// Waits for the phase `parity` of a barrier; false when `gave_up` is set or the limit is reached (which sets it).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+// Waits for the phase `parity` of a barrier; false when `gave_up` is set or the limit is reached (which sets it).  A wait
+// that spans many stages is given their count: the limit starts anew as long as that moves.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, volatile uint32_t* stages = nullptr) {
   if (bar_try(bar, parity)) return true;
-  const long long start = clock64();
+  long long start = clock64();
+  uint32_t seen = stages ? *stages : 0;
   for (;;) {
     if (bar_try(bar, parity)) return true;
     if (*gave_up) return false;
     if (clock64() - start > kWaitLimitClocks) {
-      *gave_up = 1;
-      return false;
+      const uint32_t now = stages ? *stages : seen;
+      if (now == seen) {
+        *gave_up = 1;
+        return false;
+      }
+      seen = now;
+      start = clock64();
     }
   }
 }

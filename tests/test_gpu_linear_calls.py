@@ -75,3 +75,29 @@ def test_forward_mode_tangents_are_refused():
         with torch.inference_mode():  # nothing is recorded
             assert torch.equal(linear.grouped_linear(h, w, off), want)
     assert torch.equal(linear.grouped_linear(h, w, off), want)
+
+
+def test_a_tile_may_take_longer_than_a_wait_may_stand_still():
+    """Rows of 2^30 values: one tile's sums take more than four seconds, while a wait in which nothing moves ends after two.
+    Values of +-1, whose partial sums stay far below 2^24, are summed exactly in fp32 in any order."""
+    k, n = 1 << 30, 5
+    g = gen(5)
+
+    def signs():
+        return torch.randint(0, 2, (k,), generator=g, device=DEV, dtype=torch.int8).mul_(2).sub_(1).bfloat16()
+
+    x = signs()
+    w = torch.empty(1, n, k, dtype=torch.bfloat16, device=DEV)
+    want = torch.empty(n, dtype=torch.float64, device=DEV)
+    for j in range(n):
+        w[0, j] = signs()
+        want[j] = (x * w[0, j]).sum(dtype=torch.float64)
+    same = torch.zeros(128, dtype=torch.int32, device=DEV)  # one row, read 128 times
+    off = torch.tensor([0, 128], dtype=torch.int32, device=DEV)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out = linear.grouped_linear(x[None], w, off, in_rows=same)
+    end.record()
+    linear.check_status(DEV)
+    assert torch.equal(out, want.bfloat16().expand(128, n))
+    print(f"{start.elapsed_time(end):.0f} ms")
