@@ -342,7 +342,23 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     return _product(index, x, weight, bias, activation, x_scale, weight_scale, offsets, in_rows, out_rows, out_dtype, out)
 
 
-class Int8Linear(nn.Module):
+class _Layer(nn.Module):
+    """What the layers keep wherever they are moved: weights whose rows start on 16-byte boundaries (a copy to another
+    device or type is packed, and every product would lay it out again), and biases and scales in 32 bits, as the
+    products take them, also where `half()` or `to(dtype)` change the rest of a model."""
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: self._buffers[name] for name in ("bias", "weight_scale") if self._buffers[name] is not None}
+        super()._apply(fn, recurse)
+        for name, before in kept.items():
+            now = self._buffers[name]
+            if now.dtype is not torch.float32:
+                self._buffers[name] = before.to(now.device)
+        self._buffers["weight"] = pack_rows(self._buffers["weight"])
+        return self
+
+
+class Int8Linear(_Layer):
     """A linear layer in 8 bits: `weight` `[n, k]` is quantised once, one scale per output unit; every call quantises
     its rows, one scale per row, and multiplies 8-bit integers.  The result has the type of the argument."""
 
@@ -361,7 +377,7 @@ class Int8Linear(nn.Module):
         return int8_linear(q, scale, self.weight, self.weight_scale, self.bias, self.activation, x.dtype)
 
 
-class GroupedLinear(nn.Module):
+class GroupedLinear(_Layer):
     """One linear layer per expert: `weight` `[experts, n, k]` in bfloat16 or float16, `bias` `[experts, n]`.
 
     `forward(x, offsets, in_rows, out_rows)` is `grouped_linear`.  `quantize()` turns the weights into 8 bits with one

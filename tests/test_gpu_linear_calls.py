@@ -1,4 +1,6 @@
 """GPU: the dense layers around the products: reports, gradients, modules that move, the sigmoid's ends, long rows."""
+import copy
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -101,3 +103,45 @@ def test_a_tile_may_take_longer_than_a_wait_may_stand_still():
     linear.check_status(DEV)
     assert torch.equal(out, want.bfloat16().expand(128, n))
     print(f"{start.elapsed_time(end):.0f} ms")
+
+
+def layers_of(k):
+    g = gen(k)
+    w, bias = torch.randn(3, 20, k, generator=g, device=DEV) / k ** 0.5, torch.randn(3, 20, generator=g, device=DEV)
+    return [linear.Int8Linear(w[0], bias[0], "relu"), linear.GroupedLinear(w.bfloat16(), bias, "relu"),
+            linear.GroupedLinear(w.half(), None), linear.GroupedLinear(w.bfloat16(), bias).quantize()]
+
+
+def ran(layer, k, dtype):
+    x = torch.randn(30, k, generator=gen(7), device=DEV).to(dtype)
+    if isinstance(layer, linear.Int8Linear):
+        return layer(x)
+    return layer(x, torch.tensor([0, 10, 10, 30], dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("k", [37, 64])
+@pytest.mark.parametrize("which", range(4))
+def test_layers_that_move_keep_their_layout(which, k):
+    layer = layers_of(k)[which]
+    dtype = torch.bfloat16 if layer.weight.dtype == torch.int8 else layer.weight.dtype
+    want = ran(layer, k, dtype)
+    moved = copy.deepcopy(layer).cpu().to(DEV)
+    assert linear.pack_rows(moved.weight) is moved.weight  # read in place: no copy a call
+    assert torch.equal(ran(moved, k, dtype), want)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_layers_that_change_type_keep_their_scales(which):
+    k = 37
+    layer = layers_of(k)[which]
+    before = copy.deepcopy(layer)
+    for dtype in (torch.float16, torch.bfloat16):
+        layer.to(dtype)
+        assert layer.bias is None or layer.bias.dtype == torch.float32 and torch.equal(layer.bias, before.bias)
+        scale = getattr(layer, "weight_scale")
+        assert scale is None or scale.dtype == torch.float32 and torch.equal(scale, before.weight_scale)
+        assert linear.pack_rows(layer.weight) is layer.weight
+        out = ran(layer, k, dtype)
+        assert out.dtype == dtype
+        if layer.weight.dtype == torch.int8:
+            assert torch.equal(layer.weight, before.weight) and torch.equal(out, ran(before, k, dtype))

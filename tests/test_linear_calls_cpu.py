@@ -1,7 +1,8 @@
 """CPU: the dense-layer entries' refusals and bookkeeping that need no device."""
 import pytest
+import torch
 
-from recflex_b200 import _lib
+from recflex_b200 import _lib, linear
 
 P = 1 << 20  # an aligned address that no refused call looks at
 
@@ -9,3 +10,22 @@ P = 1 << 20  # an aligned address that no refused call looks at
 @pytest.mark.parametrize("status, device", [(P + 2, 0), (P, -1), (P, 64)])
 def test_check_status_refuses(lib, status, device):
     assert lib.eb_linear_check_status(status, device, None) == _lib.EB_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(5, 37), (3, 5, 37), (5, 64)])
+def test_layers_that_move_keep_their_layout_and_scales(shape, dtype):
+    """The bookkeeping alone, without a device: a layer as its constructor leaves it."""
+    layer = linear._Layer()
+    weight = torch.arange(-60, 60).repeat(8)[: torch.Size(shape).numel()].view(shape).to(dtype)
+    layer.register_buffer("weight", linear.pack_rows(weight))
+    layer.register_buffer("weight_scale", torch.rand(shape[:-1]) / 3 if dtype is torch.int8 else None)
+    layer.register_buffer("bias", torch.rand(shape[:-1]) / 3)
+    before = {name: None if t is None else t.clone() for name, t in layer._buffers.items()}
+    for change in (lambda: layer.half(), lambda: layer.to(torch.bfloat16), lambda: layer._apply(torch.clone), lambda: layer.to("cpu")):
+        change()
+        assert linear.pack_rows(layer.weight) is layer.weight
+        assert torch.equal(layer.weight.float(), before["weight"].float())
+        assert torch.equal(layer.bias, before["bias"]) and layer.bias.dtype == torch.float32
+        assert dtype is not torch.int8 or (layer.weight.dtype == dtype and torch.equal(layer.weight_scale, before["weight_scale"]))
+    assert layer.to("meta").weight.shape == shape
