@@ -357,6 +357,18 @@ class _Layer(nn.Module):
         self._buffers["weight"] = pack_rows(self._buffers["weight"])
         return self
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        # 8-bit codes copied into 16-bit weights, or the other way round, would be no weights at all
+        given, kind = state_dict.get(prefix + "weight"), self._buffers["weight"].dtype
+        if given is not None and (given.dtype is torch.int8) != (kind is torch.int8):
+            error_msgs.append(f"{prefix}weight is {given.dtype}, the layer's is {kind}: quantise the one that is not")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        self._buffers["weight"] = pack_rows(self._buffers["weight"])  # assigned ones come in any layout and type
+        for name in ("bias", "weight_scale"):
+            if self._buffers[name] is not None:
+                self._buffers[name] = self._buffers[name].float()
+
 
 class Int8Linear(_Layer):
     """A linear layer in 8 bits: `weight` `[n, k]` is quantised once, one scale per output unit; every call quantises

@@ -29,3 +29,33 @@ def test_layers_that_move_keep_their_layout_and_scales(shape, dtype):
         assert torch.equal(layer.bias, before["bias"]) and layer.bias.dtype == torch.float32
         assert dtype is not torch.int8 or (layer.weight.dtype == dtype and torch.equal(layer.weight_scale, before["weight_scale"]))
     assert layer.to("meta").weight.shape == shape
+
+
+def layer_with(weight, scale=None):
+    layer = linear._Layer()
+    layer.register_buffer("weight", linear.pack_rows(weight))
+    layer.register_buffer("weight_scale", scale)
+    layer.register_buffer("bias", None)
+    return layer
+
+
+@pytest.mark.parametrize("strict", [False, True])
+def test_codes_are_not_loaded_as_weights(strict):
+    """An 8-bit layer's state does not fit one of 16 bits, nor the other way round, and neither is left half loaded."""
+    codes, scale = torch.arange(60, dtype=torch.int8).view(4, 15), torch.full((4,), 0.25)
+    full = (torch.arange(60).view(4, 15) / 8).bfloat16()
+    for state, layer in ((layer_with(codes, scale), layer_with(full)), (layer_with(full), layer_with(codes, scale))):
+        before = layer.weight.clone()
+        with pytest.raises(RuntimeError, match="weight is torch"):
+            layer.load_state_dict(state.state_dict(), strict=strict)
+        assert torch.equal(layer.weight, before)
+
+
+@pytest.mark.parametrize("assign", [False, True])
+def test_loaded_weights_have_the_products_layout(assign):
+    codes, scale = torch.arange(60, dtype=torch.int8).view(4, 15), torch.full((4,), 0.25)
+    layer = layer_with(torch.zeros_like(codes), torch.zeros(4))
+    layer.load_state_dict({"weight": codes, "weight_scale": scale.half()}, assign=assign)
+    assert torch.equal(layer.weight, codes) and torch.equal(layer.weight_scale, scale)
+    assert layer.weight_scale.dtype == torch.float32
+    assert linear.pack_rows(layer.weight) is layer.weight
