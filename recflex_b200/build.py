@@ -8,6 +8,7 @@ library beside the package as `recflex_b200/librecflex_b200.so`.
 from __future__ import annotations
 
 import concurrent.futures
+import contextlib
 import hashlib
 import os
 import re
@@ -82,18 +83,35 @@ def _compile(unit, force: bool, verbose: bool) -> str:
     stamp, digest = out + ".sha256", _unit_digest(unit)
     if not force and os.path.exists(out) and _read(stamp) == digest:
         return digest
-    cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", INCLUDE_DIR, "-c", os.path.join(CSRC, src), "-o", out]
+    cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", INCLUDE_DIR, "-c", os.path.join(CSRC, src)]
     if verbose:
         cmd.insert(1, "-Xptxas")
         cmd.insert(2, "-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed for {src} {extra}:\n{res.stdout}\n{res.stderr}")
+    res = _produce(cmd, out, stamp, digest, f"nvcc failed for {src} {extra}")
     if verbose:
         sys.stderr.write(res.stderr)
+    return digest
+
+
+def _produce(cmd, out: str, stamp: str, digest: str, failure: str):
+    """Run `cmd -o out` and note in `stamp` what `out` was made of.
+
+    The old note goes first and the new one comes last, and the output takes its place whole: wherever this ends, and
+    beside another process that builds, there is no note of an output that is not the one it names."""
+    fresh = f"{out}.{os.getpid()}.new"
+    with contextlib.suppress(FileNotFoundError):
+        os.remove(stamp)
+    try:
+        res = subprocess.run([*cmd, "-o", fresh], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{failure}:\n{res.stdout}\n{res.stderr}")
+        os.replace(fresh, out)
+    finally:
+        with contextlib.suppress(FileNotFoundError):
+            os.remove(fresh)
     with open(stamp, "w") as f:
         f.write(digest)
-    return digest
+    return res
 
 
 def _read(path: str) -> str:
@@ -116,12 +134,8 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
         list(pool.map(lambda u: _compile(u, force, verbose), units))
     objs = [os.path.join(BUILD_DIR, u[0]) for u in units]
-    cmd = [_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB_PATH, *objs]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-    with open(stamp, "w") as f:
-        f.write(digest)
+    cmd = [_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", *objs]
+    _produce(cmd, LIB_PATH, stamp, digest, "link failed")
     return LIB_PATH
 
 
