@@ -186,7 +186,7 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
           o[j] = fma2(make_float2((float)(int)x, (float)(int)y), mul2(row_scale, f[j]), b[j]);
         else
           o[j] = add2(make_float2(__uint_as_float(x), __uint_as_float(y)), b[j]);
-        if constexpr (SIGMOID) o[j] = make_float2(sigmoid(o[j].x), sigmoid(o[j].y));
+        if constexpr (SIGMOID) o[j] = make_float2(sigmoid<OUT == EB_OUT_F32>(o[j].x), sigmoid<OUT == EB_OUT_F32>(o[j].y));
         if constexpr (OUT == EB_OUT_F32) o[j] = make_float2(at_least(o[j].x, low), at_least(o[j].y, low));
       }
       if constexpr (OUT == EB_OUT_F32) {
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 4; ++j) {
               if (n + j >= a.n) break;
               const int64_t c = (int64_t)tile.group * a.n + n + j;
-              const float v = finish<I8>(sum[j], r, I8 ? __ldg(a.w_scale + c) : 1.0f, a.bias ? __ldg(a.bias + c) : 0.0f, a.activation);
+              const float v = finish<I8>(sum[j], r, I8 ? __ldg(a.w_scale + c) : 1.0f, a.bias ? __ldg(a.bias + c) : 0.0f, a.activation, a.out_dtype);
               store_value(a.out, (int64_t)r.dst * a.out_ld + n + j, a.out_dtype, v);
             }
           }

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kFewThreads) eb_linear_few_kernel(const __grid
     const int64_t c = (int64_t)g * a.n + n;
     store_value(a.out, (int64_t)r.dst * a.out_ld + n, a.out_dtype,
                 finish<KIND == kI8>(sum_bits<KIND>(v), r, KIND == kI8 ? __ldg(a.w_scale + c) : 1.0f,
-                                    a.bias ? __ldg(a.bias + c) : 0.0f, a.activation));
+                                    a.bias ? __ldg(a.bias + c) : 0.0f, a.activation, a.out_dtype));
   }
 }
 
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kFewThreads) eb_linear_narrow_kernel(const __g
       if (info.dst >= 0)
         store_value(a.out, (int64_t)info.dst * a.out_ld, a.out_dtype,
                     finish<KIND == kI8>(sum_bits<KIND>(v), info, KIND == kI8 ? __ldg(a.w_scale + g) : 1.0f,
-                                        a.bias ? __ldg(a.bias + g) : 0.0f, a.activation));
+                                        a.bias ? __ldg(a.bias + g) : 0.0f, a.activation, a.out_dtype));
     }
     __syncwarp();
   }

@@ -145,3 +145,18 @@ def test_layers_that_change_type_keep_their_scales(which):
         assert out.dtype == dtype
         if layer.weight.dtype == torch.int8:
             assert torch.equal(layer.weight, before.weight) and torch.equal(out, ran(before, k, dtype))
+
+
+@pytest.mark.parametrize("rows, n", [(2, 512), (40, 1), (300, 16), (900, 512), (900, 100), (65536, 1), (140, 300)])
+def test_fp32_sigmoid_to_its_last_places(rows, n):
+    """Rows of zeros give sigmoid(bias).  expf is within 2 units of the last place (2 * 2^-23 relative), the sum and the
+    quotient are rounded to nearest (2^-24 each): 3 * 2^-23 of the value, down to where fp32 itself ends (half its
+    smallest step for each of the last two roundings, two of them for expf)."""
+    bias = torch.linspace(-103, 103, n, device=DEV) if n > 1 else torch.full((1,), -88.25, device=DEV)
+    if n > 4:
+        bias[:6] = torch.tensor([0.0, float("inf"), -float("inf"), -1e4, -88.0, -87.5], device=DEV)
+    zero = torch.zeros(max(rows, n), 64, dtype=torch.int8, device=DEV)
+    scale = torch.ones(max(rows, n), device=DEV)
+    out = linear.int8_linear(zero[:rows], scale[:rows], zero[:n], scale[:n], bias, "sigmoid", torch.float32)
+    want = torch.sigmoid(bias.double()).expand(rows, n)
+    assert ((out.double() - want).abs() <= want * (3 * 2.0 ** -23) * (1 + 2.0 ** -10) + 3 * 2.0 ** -149).all()
