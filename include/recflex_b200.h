@@ -514,8 +514,9 @@ int eb_noalloc_check_status(int device, void* stream);
  * zeros has scale 0 and codes 0.  A row that holds an infinity or a NaN has
  * codes 0 and that infinity or a NaN as its scale, so that products with it are
  * NaN.  x is [rows, cols] of x_dtype (EB_OUT_*) with rows x_ld elements apart,
- * q [rows, cols] signed bytes with rows q_ld bytes apart; any alignment (rows
- * on 16-byte boundaries are read with wide loads).
+ * q [rows, cols] signed bytes with rows q_ld bytes apart; any alignment of the
+ * rows (those on 16-byte boundaries are read with wide loads), x and scale on
+ * their elements' own (EB_ERR_INVALID_ARG otherwise).
  */
 int eb_quantize_rows(const void* x, int64_t rows, int64_t cols, int64_t x_ld, int x_dtype, void* q, int64_t q_ld,
                      float* scale, int device, void* stream);

@@ -571,10 +571,11 @@ int eb_quantize_rows(const void* x, int64_t rows, int64_t cols, int64_t x_ld, in
   if (rows == 0) return EB_OK;
   if (!scale || (cols > 0 && (!x || !q))) return linear_fail(EB_ERR_INVALID_ARG, "null pointer");
   if (rows > 1 && (x_ld < cols || q_ld < cols)) return linear_fail(EB_ERR_INVALID_ARG, "rows overlap: leading dimension below %lld", (long long)cols);
+  const int64_t size = x_dtype == EB_OUT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(scale) % 4)
+    return linear_fail(EB_ERR_INVALID_ARG, "x or scale is not aligned to its elements");
   DeviceScope scope(device);
   if (!scope.ok) return linear_fail(EB_ERR_CUDA, "cannot select device %d", device);
-  const int64_t size = x_dtype == EB_OUT_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(x) % size) return linear_fail(EB_ERR_INVALID_ARG, "x is not aligned to its elements");
   QuantArgs a;
   a.x = x;
   a.q = static_cast<int8_t*>(q);

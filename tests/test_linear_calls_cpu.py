@@ -59,3 +59,9 @@ def test_loaded_weights_have_the_products_layout(assign):
     assert torch.equal(layer.weight, codes) and torch.equal(layer.weight_scale, scale)
     assert layer.weight_scale.dtype == torch.float32
     assert linear.pack_rows(layer.weight) is layer.weight
+
+
+@pytest.mark.parametrize("x, scale, dtype", [(P, P + 2, _lib.EB_OUT_BF16), (P, P + 1, _lib.EB_OUT_F32),
+                                             (P + 1, P, _lib.EB_OUT_F16), (P + 2, P, _lib.EB_OUT_F32)])
+def test_quantize_rows_refuses_addresses_off_their_elements(lib, x, scale, dtype):
+    assert lib.eb_quantize_rows(x, 4, 8, 8, dtype, P, 16, scale, 0, None) == _lib.EB_ERR_INVALID_ARG
