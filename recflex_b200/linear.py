@@ -166,6 +166,8 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 @functools.lru_cache(maxsize=256)
 def _group_workspace(rows: int, num_groups: int) -> int:
     """Bytes of scratch that eb_group_rows needs for these sizes."""
+    if not -2 ** 31 <= num_groups < 2 ** 31:  # ctypes would keep its low half
+        raise ValueError(f"num_groups must lie in [1, {MAX_GROUPS}], got {num_groups}")
     need = C.c_size_t()
     _lib.check(_lib.load().eb_group_rows_workspace_bytes(rows, num_groups, C.byref(need)))
     return need.value

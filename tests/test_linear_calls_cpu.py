@@ -65,3 +65,13 @@ def test_loaded_weights_have_the_products_layout(assign):
                                              (P + 1, P, _lib.EB_OUT_F16), (P + 2, P, _lib.EB_OUT_F32)])
 def test_quantize_rows_refuses_addresses_off_their_elements(lib, x, scale, dtype):
     assert lib.eb_quantize_rows(x, 4, 8, 8, dtype, P, 16, scale, 0, None) == _lib.EB_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("num_groups", [2 ** 32 + 3, 2 ** 31, -2 ** 31 - 1, 2 ** 64 + 1])
+def test_expert_counts_that_do_not_fit_the_entry_are_refused(lib, num_groups):
+    """ctypes keeps the low half of a number, which may be a count that the entry takes."""
+    with pytest.raises(ValueError, match="num_groups"):
+        linear._group_workspace(16, num_groups)
+    for count in (0, -1, 1025):
+        with pytest.raises(_lib.EbError):
+            linear._group_workspace(16, count)
