@@ -18,6 +18,7 @@ from typing import Optional, Tuple
 import torch
 import torch.autograd.forward_ad as _forward_ad
 import torch.nn as nn
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import _lib
 
@@ -250,7 +251,8 @@ def _product(index, x, weight, bias, activation, x_scale, weight_scale, offsets,
     if out_code is None:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     zero_rest = 0
-    if out is None:
+    given = out is not None
+    if not given:
         # Rows on 16-byte boundaries, as the next product reads them and the tiles store them (int8 65536 x 256 x 431:
         # 21 us, packed 86); up to 16 units, where the gaps would be a good part of the result, they are packed.
         per_out = 16 // out_dtype.itemsize
@@ -302,6 +304,8 @@ def _product(index, x, weight, bias, activation, x_scale, weight_scale, offsets,
     code = _lib.load().eb_linear(args, index, _current_stream(index))
     if code:
         _lib.check(code)
+    if given:  # what autograd has saved of it is no longer what it was
+        _increment_version(out)
     return out
 
 

@@ -160,3 +160,20 @@ def test_fp32_sigmoid_to_its_last_places(rows, n):
     out = linear.int8_linear(zero[:rows], scale[:rows], zero[:n], scale[:n], bias, "sigmoid", torch.float32)
     want = torch.sigmoid(bias.double()).expand(rows, n)
     assert ((out.double() - want).abs() <= want * (3 * 2.0 ** -23) * (1 + 2.0 ** -10) + 3 * 2.0 ** -149).all()
+
+
+def test_a_given_out_counts_as_changed():
+    """What autograd has saved of `out` is no longer what it was: a backward pass through it must say so."""
+    a = torch.ones(8, 16, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    x = torch.randn(8, 32, generator=gen(3), device=DEV).bfloat16()
+    w = torch.randn(1, 16, 32, generator=gen(4), device=DEV).bfloat16()
+    off = torch.tensor([0, 8], dtype=torch.int32, device=DEV)
+    wide = torch.ones(8, 20, device=DEV, dtype=torch.bfloat16)
+    for out in (torch.ones(8, 16, device=DEV, dtype=torch.bfloat16), wide[:, :16]):
+        y = (a * out).sum()
+        linear.grouped_linear(x, w, off, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        out = torch.ones(8, 16, device=DEV, dtype=torch.bfloat16)
+        assert linear.grouped_linear(x, w, off, out=out) is out
