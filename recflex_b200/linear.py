@@ -62,8 +62,8 @@ def check_status(device=None) -> None:
 
 _Tensor = torch.Tensor
 _I8, _I32 = (torch.int8,), (torch.int32,)
-# the current stream's handle by device index, without the stream object around it
-_current_stream = torch._C._cuda_getCurrentRawStream
+# the current stream's handle by device index, without the stream object around it (not there in a torch without CUDA)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _check(name: str, t: torch.Tensor, dims: int, dtypes, index: Optional[int] = None) -> int:

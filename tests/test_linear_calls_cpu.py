@@ -1,9 +1,14 @@
 """CPU: the dense-layer entries' refusals and bookkeeping that need no device."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from recflex_b200 import _lib, linear
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = 1 << 20  # an aligned address that no refused call looks at
 
 
@@ -75,3 +80,11 @@ def test_expert_counts_that_do_not_fit_the_entry_are_refused(lib, num_groups):
     for count in (0, -1, 1025):
         with pytest.raises(_lib.EbError):
             linear._group_workspace(16, count)
+
+
+def test_the_package_is_imported_without_cuda_in_torch():
+    """The parsers, schedules and modules' definitions need no device, nor a torch that has one."""
+    code = ("import torch\ndel torch._C._cuda_getCurrentRawStream\n"
+            "import recflex_b200.rec_modules, recflex_b200.linear\n")
+    res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-1500:]
