@@ -582,7 +582,8 @@ int eb_linear(const eb_linear_args* args, int device, void* stream);
 
 /* Reads and clears the status word of eb_linear, both at once: EB_ERR_BAD_INPUT for bad offsets or row numbers,
  * EB_ERR_CUDA when a kernel gave up waiting for its own copies.  Synchronises `stream`, and answers for the products in
- * front of it there; what a product on another stream reports later stays in the word for the next check. */
+ * front of it there; what a product on another stream reports later stays in the word for the next check.
+ * EB_ERR_UNSUPPORTED while `stream` is being captured. */
 int eb_linear_check_status(uint32_t* status, int device, void* stream);
 
 /* Message of the calling thread's last failure ("" if none). */

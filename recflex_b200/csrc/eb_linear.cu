@@ -906,6 +906,9 @@ int eb_linear_check_status(uint32_t* status, int device, void* stream) {
   DeviceScope scope(device);
   if (!scope.ok) return linear_fail(EB_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
+    return linear_fail(EB_ERR_UNSUPPORTED, "the status word cannot be read while the stream is being captured");
   std::lock_guard<std::mutex> lock(g_found_lock[device]);
   uint32_t host = 0;
   take_status_kernel<<<1, 1, 0, st>>>(status);

@@ -177,3 +177,21 @@ def test_a_given_out_counts_as_changed():
     with torch.inference_mode():
         out = torch.ones(8, 16, device=DEV, dtype=torch.bfloat16)
         assert linear.grouped_linear(x, w, off, out=out) is out
+
+
+def test_a_check_during_a_capture_is_refused_and_leaves_the_capture_alone():
+    g = gen(6)
+    x, w = torch.randn(40, 32, generator=g, device=DEV).half(), torch.randn(2, 16, 32, generator=g, device=DEV).half()
+    off = torch.tensor([0, 15, 40], dtype=torch.int32, device=DEV)
+    want = linear.grouped_linear(x, w, off)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = linear.grouped_linear(x, w, off)
+        with pytest.raises(_lib.EbError) as e:
+            linear.check_status(DEV)
+        second = linear.grouped_linear(x, w, off)
+    assert e.value.code == _lib.EB_ERR_UNSUPPORTED
+    graph.replay()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    linear.check_status(DEV)
