@@ -75,6 +75,7 @@ struct LinearArgs {
   int cluster;  // CTAs of a cluster: CG, or the number of pieces that K is split into
   int align;    // rows of out start on multiples of 16, 4 or 2 bytes
   int boxes;    // results go out in boxes of 32 rows (map_out), where a warp has that many: rows in order, align 16
+  int box_cols; // columns that the boxes store: tensor copies write whole 16 bytes, also where the tensor ends inside them
 };
 
 struct Tile {
@@ -158,13 +159,14 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
       to[i] = dst < 0 ? nullptr : static_cast<uint8_t*>(a.out) + ((int64_t)dst * a.out_ld + n) * kSize + piece * 16;
     }
   }
+  uint32_t mine = staging;
 #pragma unroll 1
   for (int c = 0; c < SPAN && n + c < a.n; c += kUnit) {
     uint32_t v[kUnit];
     tmem_load(tm + c, v);
     if (elect_one()) store_wait_read<BUFFERS - 1>();
     __syncwarp();  // this buffer's results have been read
-    const uint32_t mine = staging + buffer;
+    mine = staging + buffer;
     tmem_wait_load();
     if (any_zero && r.zero) {  // products of a row number outside x: zeros (at 8 bits their factor is 0)
 #pragma unroll
@@ -199,8 +201,10 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
     if constexpr (BOX) {
       fence_copies();
       __syncwarp();
-      if (elect_one()) store_2d(map_out, n + c, first_row, mine);
-      if (BUFFERS > 1) buffer ^= 32 * kStagingRow;
+      if (n + c < args.box_cols) {
+        if (elect_one()) store_2d(map_out, n + c, first_row, mine);
+        if (BUFFERS > 1) buffer ^= 32 * kStagingRow;
+      }
     } else {
       __syncwarp();
       if (args.align == 16 || SPAN < 32) {
@@ -250,6 +254,20 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
             *reinterpret_cast<uint16_t*>(out) = w;
           }
         }
+      }
+    }
+  }
+  if constexpr (BOX) {
+    // the last columns fill no 16 bytes: each lane stores those of its own row, from what the last unit left
+    const int rest = args.box_cols - n, left = (a.n - args.box_cols) * kSize;
+    if (left && rest >= 0 && rest < SPAN) {
+      const uint4 w = shared_read(mine + place(lane, rest % kUnit / kElems));
+      uint8_t* at = static_cast<uint8_t*>(a.out) + ((int64_t)(first_row + lane) * a.out_ld + args.box_cols) * kSize;
+      if (left & 8) *reinterpret_cast<uint2*>(at) = make_uint2(w.x, w.y);
+      if (left & 4) *reinterpret_cast<uint32_t*>(at + (left & 8)) = left & 8 ? w.z : w.x;
+      if (left & 2) {
+        const uint32_t last = left & 8 ? (left & 4 ? w.w : w.z) : (left & 4 ? w.y : w.x);
+        *reinterpret_cast<uint16_t*>(at + (left & 12)) = (uint16_t)last;
       }
     }
   }
@@ -704,8 +722,9 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// A [groups, rows, k] tensor of `dtype` in boxes of `box_rows` rows x `box_bytes` (128 or 64, swizzled as wide); what lies
-// outside reads as zeros and is not written.
+// A [groups, rows, k] tensor of `dtype` in boxes of `box_rows` rows x `box_bytes` (128 or 64, swizzled as wide).  What lies
+// outside reads as zeros and is not written, except that writes go on to the end of the 16 bytes that a row ends in: a
+// tensor to be written has rows of whole 16 bytes.
 bool make_map(CUtensorMap* map, int dims, int dtype, const void* p, int64_t k, int64_t rows, int64_t ld, int64_t groups,
               int64_t group_ld, int box_rows, int box_bytes = kKBytes) {
   const int size = dtype == EB_ROW_I8 ? 1 : dtype == EB_OUT_F32 ? 4 : 2;
@@ -740,8 +759,9 @@ int launch(LinearArgs& args, int device, int sms, int64_t m_tiles, int split, cu
   // a unit of columns of 32 rows; tiles whose unit is narrower than a staging row store row by row
   constexpr int kSpan = S::kPart >= 64 ? S::kPart / 2 : S::kPart;
   const int size = a.out_dtype == EB_OUT_F32 ? 4 : 2;
-  args.boxes = !SPLIT && args.align == 16 && !a.out_rows && kSpan * size >= kStagingRow &&
-               make_map(&map_out, 2, a.out_dtype, a.out, a.n, a.out_rows_total, a.out_ld, 1, 0, 32, kStagingRow);
+  args.box_cols = (int)((int64_t)a.n * size / 16 * 16 / size);
+  args.boxes = !SPLIT && args.align == 16 && !a.out_rows && kSpan * size >= kStagingRow && args.box_cols > 0 &&
+               make_map(&map_out, 2, a.out_dtype, a.out, args.box_cols, a.out_rows_total, a.out_ld, 1, 0, 32, kStagingRow);
   const auto kernel = eb_linear_kernel<I8, BN, CG, SPLIT>;
   static std::atomic<uint64_t> ready{0};  // devices whose copy of the kernel may use this much shared memory
   if (!(ready.load() >> device & 1)) {

@@ -136,7 +136,8 @@ __device__ __forceinline__ void load_rows4(uint32_t dst, const CUtensorMap* map,
 
 // Shared memory that this thread's CTA wrote becomes visible to tensor copies issued after a barrier.
 __device__ __forceinline__ void fence_copies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// A box of a 2-D tensor from shared memory; what lies outside the tensor is not written.
+// A box of a 2-D tensor from shared memory; what lies outside the tensor is not written, but for the rest of the 16 bytes
+// in which a row ends.
 __device__ __forceinline__ void store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");

@@ -195,3 +195,31 @@ def test_a_check_during_a_capture_is_refused_and_leaves_the_capture_alone():
     graph.replay()
     assert torch.equal(first, want) and torch.equal(second, want)
     linear.check_status(DEV)
+
+
+@pytest.mark.parametrize("kind", ["i8", "bf16"])
+@pytest.mark.parametrize("n", [1, 17, 33, 100, 250, 431, 1001])
+@pytest.mark.parametrize("rows, k", [(3, 200), (300, 200), (300, 9000), (9000, 1000)])
+def test_nothing_is_written_beside_the_columns_of_a_wide_out(rows, k, n, kind):
+    """Rows on 16-byte boundaries with columns behind the last one, and rows behind the last one, stay as they were."""
+    g = gen(rows + n)
+    x = torch.randn(rows, k, generator=g, device=DEV)
+    w = torch.randn(n, k, generator=g, device=DEV) / k ** 0.5
+    perm = torch.randperm(rows, generator=g, device=DEV).to(torch.int32)
+    off = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device=DEV)
+    if kind == "i8":
+        (q, s), (wq, ws) = linear.quantize_rows(x), linear.quantize_rows(w)
+        calls = [(dtype, lambda out, dtype=dtype: linear.int8_linear(q, s, wq, ws, None, "relu", dtype, out=out))
+                 for dtype in (torch.float32, torch.bfloat16, torch.float16)]
+    else:
+        h, two = x.bfloat16(), torch.stack([w, -w]).bfloat16()
+        calls = [(torch.bfloat16, lambda out, rows=rows: linear.grouped_linear(h, two, off, out_rows=rows, out=out)) for rows in (None, perm)]
+    for dtype, call in calls:
+        packed = torch.empty(rows, n, dtype=dtype, device=DEV)
+        call(packed)
+        for wide in (1024, 1027):
+            full = torch.full((rows + 40, wide), 7.0, dtype=dtype, device=DEV)
+            call(full[:, :n])
+            assert torch.equal(full[:rows, :n], packed)
+            assert (full[:, n:] == 7).all() and (full[rows:] == 7).all()
+    linear.check_status(DEV)
