@@ -223,3 +223,36 @@ def test_nothing_is_written_beside_the_columns_of_a_wide_out(rows, k, n, kind):
             assert torch.equal(full[:rows, :n], packed)
             assert (full[:, n:] == 7).all() and (full[rows:] == 7).all()
     linear.check_status(DEV)
+
+
+# sizes that reach each of the kernels and tiles, in rows that end inside 16 bytes
+SIZES = [(1, 37, 40), (3, 1001, 33), (40, 37, 1), (300, 203, 1), (200, 3001, 5), (300, 203, 17), (300, 9001, 300), (4096, 1923, 333),
+         (4096, 1923, 1000), (4096, 483, 1000), (9000, 6001, 1000), (700, 15607, 700), (16300, 3003, 1001)]
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("kind", ["i8", "bf16", "f16"])
+@pytest.mark.parametrize("rows, k, n", SIZES)
+def test_what_stands_behind_the_columns_is_not_multiplied(rows, k, n, kind, gather):
+    """Columns behind k in the storage of x and the weights: the largest codes or NaN change nothing."""
+    g = gen(rows + k)
+    dtype = {"i8": torch.int8, "bf16": torch.bfloat16, "f16": torch.float16}[kind]
+
+    def made(*shape):
+        t = torch.randn(*shape, generator=g, device=DEV)
+        return (t * 40).clamp(-127, 127).to(dtype) if kind == "i8" else t.to(dtype)
+
+    pitch = (k + 15) // 16 * 16 + 32
+    x, w = made(rows, pitch), made(3, n, pitch)
+    kw = dict(x_scale=torch.rand(rows, generator=g, device=DEV), weight_scale=torch.rand(3, n, generator=g, device=DEV)) if kind == "i8" else {}
+    ids = torch.randint(0, 3, (rows,), generator=g, device=DEV)
+    order, off = linear.group_rows(ids, 3)
+    got = []
+    for poison in (0, 127 if kind == "i8" else float("nan")):
+        x[:, k:], w[:, :, k:] = poison, poison
+        got.append(linear.grouped_linear(x[:, :k], w[:, :, :k], off, in_rows=order if gather else None, **kw).clone())
+        if kind == "i8":
+            got.append(linear.int8_linear(x[:, :k], kw["x_scale"], w[0, :, :k], kw["weight_scale"][0]).clone())
+    half = len(got) // 2
+    for a, b in zip(got[:half], got[half:]):
+        assert torch.equal(a, b)
