@@ -12,14 +12,17 @@
 // whole row segments are stored, wherever their rows go.  Which tiles there are
 // follows from the offsets on the GPU; the host never reads them.
 //
-// What bounds it.  At long K the bandwidth of shared memory: products of
-// 256 x 256 x 32 bytes read 96 bytes a clock and SM, and the copies write 47
-// (512-column tiles) to 64 (256) beside them, of 128; the tensor pipes are 83 to
-// 88 % active (int8 16384 x 15608 x 1024 in 0.169 ms, 3.1 Pop/s; bf16 of that
-// size in 8 groups, rows by index, 0.395 ms, 1.33 Pflop/s).  At short K the
-// results' way out (65536 x 480 x 1024 in int8: 43 us, 3.9 TB/s), and in small
-// products the way from launch to the first copies and from the last product to
-// the stored results, about 8 us of int8 4096 x 1924 x 1024's 12.7.
+// What bounds it (times on the device, repeated on one set of inputs).  At long
+// K the bandwidth of shared memory: products of 256 x 256 x 32 bytes read 96
+// bytes a clock and SM, and the copies write 47 (512-column tiles) to 64 (256)
+// beside them, of 128; the tensor pipes are 82 to 86 % active (int8
+// 16384 x 15608 x 1024 in 0.166 ms, 3.2 Pop/s; bf16 of that size in 8 groups,
+// rows by index, 0.385 ms, 1.36 Pflop/s; call after call on changing inputs the
+// power cap holds them to 0.199 ms, 2.6 Pop/s, and 0.473 ms, 1.11 Pflop/s).  At
+// short K the results' way out (65536 x 480 x 1024 in int8: 42 us, 3.9 TB/s),
+// and in small products the way from launch to the first copies and from the
+// last product to the stored results, about 8 us of int8 4096 x 1924 x 1024's
+// 12.7.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -234,8 +237,8 @@ __device__ __forceinline__ void store_span(const LinearArgs& args, const CUtenso
           }
         }
       } else {
-        // rows on no 16-byte boundaries: neighbouring lanes store neighbouring words (or 16-bit values) of a row.  Values
-        // one by one from the 16-byte pieces took 125 us for int8 30000 x 2000 x 700, whose products take 46.
+        // rows on no 16-byte boundaries: neighbouring lanes store neighbouring words (or 16-bit values) of a row.  Packed
+        // rows cost: int8 65536 x 256 x 431 to bf16 takes 86 us so and 21 into rows on such boundaries.
         const int log_each = args.align >= 4 ? 2 : 1, per_row = kStagingRow >> log_each;
         const int at = lane % per_row << log_each;  // bytes into the staging row
         const int left = a.n - (n + c) - at / kSize;
@@ -793,21 +796,26 @@ int dispatch(LinearArgs& args, int device, cudaStream_t st) {
   const int sms = sm_count(device);
   if (sms < 2) return linear_fail(EB_ERR_CUDA, "cannot read the SM count of device %d", device);
   args.k_steps = (int)(((int64_t)a.k * (I8 ? 1 : 2) + kKBytes - 1) / kKBytes);
-  // A few rows: one row of 15608 x 1024 takes 6.2 us in int8 (tiles with K split over 4 CTAs: 11.5), four 9.5 (12.0),
-  // eight 15.3 (11.2); six rows over 16 experts of 1924 x 1024 in fp16 9.1 (12.0), 32 over 64 22.4 (27.8), 64 over 64
-  // 52 (28): at most four rows, or half as many as there are experts.
+  // A few rows: one row of 15608 x 1024 takes 5.4 us in int8 (tiles with K split over 4 CTAs: 11.3), four 8.9 (11.7),
+  // eight 13.5 (11.7); six rows over 16 experts of 1924 x 1024 in fp16 8.3 (11.6), 32 over 64 28 (26), 64 over 64 67 (48):
+  // at most four rows, or half as many as there are experts.  The host knows no more than these two numbers: 512 rows over
+  // 1024 experts of 1924 x 256 take 178 (112), and 136 (37) where all of them chose one expert, whose weights are then
+  // read for every few of its rows.
   if (a.positions <= 4 || 2 * a.positions <= a.num_groups) return launch_few(a, sms, st);
-  // One unit over rows of up to 256 bytes: 65536 rows of 128 int8 take 5.0 us (16-column tiles: 9.1), of 512 15.4 (9.9).
+  // One unit over rows of up to 256 bytes: 65536 rows of 128 int8 take 4.6 us (16-column tiles: 6.8), of 256 7.2 (7.2),
+  // of 512 11.7 (8.1).
   if (a.n == 1 && (int64_t)a.k * (I8 ? 1 : 2) <= 256) return launch_narrow(a, sms, st);
   const int64_t m128 = row_tiles(a, 128), m256 = row_tiles(a, 256);
+  // Up to 16 units one tile a 128 rows, by one CTA over all of K: x is read once.  Few rows of long K leave most SMs idle so
+  // (5 or 128 rows of 24160 x 16 in int8 32 us; 4096 of 15608 23).
   if (a.n <= 16) return launch<I8, 16, 1, false>(args, device, sms, m128, 1, st);
   // The tile with the least estimated time: full waves of tiles (every group ends half a tile into its last one, on
   // average) at so many clocks per stage of K, plus the clocks that a tile costs beside its products, plus those of
   // storing the last one.  Wide tiles read x and the weights less often from L2, which bounds them; narrow ones give all
   // SMs work.  Rows by index cannot be copied faster than 350 to 850 clocks a stage for few to 128.  Clocks fitted to 38
   // measured products (256 to 65536 rows, 256 to 15608 columns, 128 to 1024 units, 1 to 64 groups, int8 and 16 bits); on
-  // 240 products of random sizes the choice is 0.8 % behind the fastest tile on average.  Each of the five is the fastest
-  // for some, and up to three times as slow as the fastest for others.
+  // 240 products of random sizes above 16 units and 4 rows the choice was 0.8 % behind the fastest tile on average.  Each of
+  // the five is the fastest for some, and up to three times as slow as the fastest for others.
   struct Choice {
     int rows, cols, ctas, stage, tile, last;
   };

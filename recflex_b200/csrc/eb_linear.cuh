@@ -10,7 +10,8 @@
 namespace ebk {
 
 // Offsets made non-decreasing inside [0, positions], and the number of row tiles in front of each group.  Called by
-// one whole warp.
+// one whole warp, 32 groups a turn (8192 rows of 1024 x 256 in bf16: 8 experts 11 us, 64 15, 512 73, 1024 127, of which
+// their weights' bytes are 1, 5, 41 and 82).
 __device__ __forceinline__ void groups_of(const eb_linear_args& a, int* off, int* tiles, int tile_rows, uint32_t* bad) {
   const int lane = threadIdx.x % 32;
   const int P = (int)a.positions;
@@ -143,7 +144,8 @@ __device__ __forceinline__ float finish(uint32_t bits, const RowInfo& r, float c
   return activate(v, act, out_dtype);
 }
 
-// Rows of zeros for the positions of no group, by `threads` threads of every CTA.
+// Rows of zeros for the positions of no group, by `threads` threads of every CTA, value by value in front of the first tile:
+// bf16 65536 x 256 x 1024 takes 45 us with all rows in groups, 86 with a tenth of them in none, 249 with half.
 __device__ __forceinline__ void zero_rest(const eb_linear_args& a, const int* off, int64_t thread, int64_t threads) {
   const int64_t group_rows = off[a.num_groups] - off[0];
   const int64_t rest = (a.positions - group_rows) * a.n;

@@ -73,8 +73,8 @@ __device__ __forceinline__ const uint8_t* row_of(const eb_linear_args& a, int p,
 
 // A CTA per run of units and tile of ROWS positions of one group; `share` of its warps split K, each set of warps takes 4
 // units.  Bound by the weights' bytes: each lane keeps 8 weight loads in flight, the rows of x come from L1 / L2.  One
-// row of 15608 x 1024 takes 5.4 us in int8 (3.0 TB/s, launch included) and 8.0 in fp16 (4.0 TB/s); six rows over 16
-// experts of 1924 x 1024 in bf16 8.6.
+// row of 15608 x 1024 takes 5.4 us in int8 (3.0 TB/s, launch included) and 7.1 in fp16 (4.5 TB/s); six rows over 16
+// experts of 1924 x 1024 in bf16 8.4.
 template <Kind KIND, int ROWS>
 __global__ void __launch_bounds__(kFewThreads) eb_linear_few_kernel(const __grid_constant__ eb_linear_args a, int share) {
   constexpr int kSize = KIND == kI8 ? 1 : 2, kPer = 16 / kSize;
