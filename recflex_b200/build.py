@@ -115,10 +115,11 @@ def _produce(cmd, out: str, stamp: str, digest: str, failure: str):
 
 
 def _read(path: str) -> str:
-    if not os.path.exists(path):
+    try:
+        with open(path) as f:
+            return f.read().strip()
+    except FileNotFoundError:  # never there, or taken away just now by another process that builds
         return ""
-    with open(path) as f:
-        return f.read().strip()
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> str:

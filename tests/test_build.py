@@ -127,3 +127,10 @@ def test_a_link_that_broke_off_is_done_again(tree, monkeypatch):
     build.build()
     assert library(tree) == good
     assert not [f for f in os.listdir(tree / "build") if f not in ("a.o", "b.o", "a.o.sha256", "b.o.sha256", "sources.sha256")]
+
+
+def test_a_note_that_goes_away_while_it_is_read_is_no_note(tree, monkeypatch):
+    """Another process takes the notes away when it begins to build."""
+    build.build()
+    monkeypatch.setattr(build.os.path, "exists", lambda path: True)
+    assert build._read(str(tree / "build" / "gone.sha256")) == ""
