@@ -77,8 +77,9 @@ __device__ __forceinline__ float at_least(float v, float low) {
 }
 // 1 / (1 + e^-v), for v < 0 as e^v / (1 + e^v): e^-|v| neither overflows nor loses the smallest values.  expf is within 2
 // units of the last place.  Results in 32 bits take the IEEE quotient (3 units in all, down to the smallest subnormal),
-// results in 16 bits __fdividef (5 units, far inside their rounding).  int8 65536 x 256 x 432 takes 37 us in bf16 (without
-// a sigmoid 21) and 78 in fp32 (26); the scores of 65536 rows of 128 in fp32 4.6 with it and without.
+// results in 16 bits __fdividef (5 units, far inside their rounding).  int8 65536 x 256 x 432 takes 38 us in bf16 (without
+// a sigmoid 21) and 79 in fp32 (26; with __fdividef 43, off by up to 2.0 units between -10 and 0 where this is by 1.75); the
+// scores of 65536 rows of 128 in fp32 4.6 with it and without.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid(float v) {
   const float e = expf(-fabsf(v)), top = v < 0.0f ? e : 1.0f;
